@@ -295,6 +295,40 @@ int scree_varlen_softmax_bwd(const void* y, const void* dy, void* dx, const int3
                              int batch, int64_t total_tokens, int64_t features, int dtype,
                              void* stream);
 
+/* ------------------------------------------------------ token log probabilities
+ * Per row of `vocab` logits (rows `row_stride` elements apart, any alignment;
+ * rows * ceil(vocab / 16384) at most 2^23) and its given token:
+ *   logprob = log_softmax(row)[target], entropy = that of softmax(row),
+ *   top_logprob / top_index (rows, top_k): the top_k (0 to 64) largest
+ *   log_softmax values, falling, the lowest index first among equal logits.
+ * All but top_index are fp32, for every logit dtype.  `targets` are integers of
+ * `target_bytes` (4 or 8) bytes: a negative one means the row has none (its
+ * logprob is 0 and has no gradient), one past the vocabulary makes the row's
+ * logprob and gradient NaN.  Logits of -inf have probability zero; a row that
+ * holds NaN or +inf, or only -inf, has NaN results (top_index stays in range).
+ * `stats` (rows, 2) fp32, may be NULL, receives what the backward needs.  No
+ * counterpart in the reference. */
+
+/* Bytes of workspace for scree_token_logprobs (0 when none is needed): few
+ * rows are split over workgroups whose partial results are joined. */
+size_t scree_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
+
+int scree_token_logprobs(const void* logits, int64_t row_stride, const void* targets,
+                         int target_bytes, int64_t rows, int64_t vocab, int top_k, float* logprob,
+                         float* entropy, float* stats, float* top_logprob, int64_t* top_index,
+                         int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dlogits (rows `dlogits_stride` elements apart) from the gradients of the
+ * three outputs, each of which may be NULL (zero), and the forward's logits,
+ * targets, stats, entropy and top_index.  A row whose gradients are all zero
+ * (no target, for one) gets zeros whatever its logits. */
+int scree_token_logprobs_bwd(const void* logits, int64_t row_stride, const void* targets,
+                             int target_bytes, int64_t rows, int64_t vocab, int top_k,
+                             const float* stats, const float* entropy, const int64_t* top_index,
+                             const float* dlogprob, const float* dentropy,
+                             const float* dtop_logprob, void* dlogits, int64_t dlogits_stride,
+                             int dtype, void* stream);
+
 /* ------------------------------------------------------------ padded <-> packed
  * Replace the host loops of scree.to_padded / scree.from_padded
  * (src/scree/_core.py:161-266 and :269-301; torch branch :240-266 and

@@ -113,5 +113,29 @@ def varlen_softmax(arr: Array) -> Array:
     return Array._trusted(varlen_softmax_hip(arr.values, arr.offsets), arr.offsets, 0)
 
 
+def varlen_token_logprobs(logits: Array, targets, top_k: int = 0):
+    """Log probabilities of given tokens under packed ``(total, vocab)`` logits.
+
+    ``targets`` is an :class:`Array` with the same offsets or a tensor of one
+    token per row.  Returns a ``TokenLogprobs`` of Arrays: ``logprob``,
+    ``entropy`` and, for ``top_k`` > 0, ``top_logprob`` and ``top_index``
+    (else None); see :func:`scree_amd.kernels.hip.varlen_token_logprobs_hip`.
+    No counterpart in the reference.
+    """
+    import torch
+
+    from .hip import TokenLogprobs, varlen_token_logprobs_hip
+
+    if logits.ragged_dim != 0:
+        raise NotImplementedError("varlen_token_logprobs supports ragged_dim=0 only")
+    _require_device(logits.values, "varlen_token_logprobs")
+    if isinstance(targets, Array):
+        if targets.offsets is not logits.offsets and not torch.equal(targets.offsets, logits.offsets):
+            raise ValueError("logits and targets must have identical offsets")
+        targets = targets.values
+    out = varlen_token_logprobs_hip(logits.values, targets, top_k)
+    return TokenLogprobs(*[None if t is None else Array._trusted(t, logits.offsets, 0) for t in out])
+
+
 __all__ = ["varlen_add_rmsnorm", "varlen_attention", "varlen_layernorm", "varlen_rmsnorm",
-           "varlen_softmax"]
+           "varlen_softmax", "varlen_token_logprobs"]

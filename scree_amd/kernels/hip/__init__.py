@@ -22,6 +22,11 @@ from .attention import (
     varlen_attention_hip,
     varlen_attention_hip_backward,
 )
+from .logprobs import (
+    TokenLogprobs,
+    varlen_token_logprobs_hip,
+    varlen_token_logprobs_hip_backward,
+)
 from .norms import (
     varlen_add_rmsnorm_hip,
     varlen_add_rmsnorm_hip_backward,
@@ -50,6 +55,7 @@ __all__ = [
     "TRITON_AVAILABLE",
     "HipUnavailableError",
     "ScreeHipError",
+    "TokenLogprobs",
     "VarlenAttentionHip",
     "attention_schedule",
     "needs_schedule",
@@ -68,6 +74,8 @@ __all__ = [
     "varlen_rmsnorm_hip_backward",
     "varlen_softmax_hip",
     "varlen_softmax_hip_backward",
+    "varlen_token_logprobs_hip",
+    "varlen_token_logprobs_hip_backward",
     "varlen_attention_triton",
     "varlen_attention_triton_autograd",
     "varlen_attention_triton_backward",

@@ -1,0 +1,148 @@
+"""Log probabilities of given tokens on the HIP kernels: the loss and scoring
+end of a packed language-model step.
+
+No counterpart in the reference.  For every row of packed ``logits`` and its
+given token :func:`varlen_token_logprobs_hip` returns the token's log
+probability, the entropy of the row's distribution and, on request, its most
+likely tokens, from one pass over the logits.  The call is autograd-aware; the
+backward (:func:`varlen_token_logprobs_hip_backward`) reads the logits again
+and writes their gradient, no probabilities are kept.
+"""
+
+from __future__ import annotations
+
+import functools
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _ffi
+
+MAX_TOP_K = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprob`` and ``entropy`` ``(total,)`` fp32; ``top_logprob`` fp32 and
+    ``top_index`` int64 ``(total, top_k)``, None for ``top_k = 0``."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: Optional[torch.Tensor]
+    top_index: Optional[torch.Tensor]
+
+
+def _check(logits, targets, top_k):
+    assert logits.is_cuda, "varlen_token_logprobs on HIP requires ROCm device tensors"
+    assert logits.dim() == 2 and logits.shape[1] >= 1, "logits must be (total_tokens, vocab)"
+    assert logits.dtype in (torch.float32, torch.float16, torch.bfloat16), (
+        f"unsupported dtype {logits.dtype}")
+    assert targets.shape == logits.shape[:1], "targets must have one token per row of logits"
+    assert targets.dtype in (torch.int32, torch.int64), "targets must be int32 or int64"
+    assert targets.device == logits.device, "targets must be on the same device as logits"
+    assert 0 <= top_k <= min(MAX_TOP_K, logits.shape[1]), (
+        f"top_k must be in [0, {MAX_TOP_K}] and at most the vocabulary")
+
+
+def _rows_view(x):
+    """``x`` itself when its rows can be read in place, else a contiguous copy."""
+    ok = x.shape[1] == 1 or x.stride(1) == 1
+    return x if ok and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows, vocab, top_k):
+    return int(_ffi.lib().scree_token_logprobs_workspace_bytes(rows, vocab, top_k))
+
+
+def logprobs_fwd(x, targets, top_k, want_stats):
+    rows, vocab = x.shape
+    dev = x.device
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(logprob)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
+    top_lp = top_i = None
+    if top_k:
+        top_lp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+        top_i = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    if rows:
+        nbytes = _workspace_bytes(rows, vocab, top_k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _ffi.launch(_ffi.lib().scree_token_logprobs, x, x.data_ptr(), x.stride(0),
+                    targets.data_ptr(), targets.element_size(), rows, vocab, top_k,
+                    logprob.data_ptr(), entropy.data_ptr(), _ffi.ptr(stats), _ffi.ptr(top_lp),
+                    _ffi.ptr(top_i), _ffi.dtype_code(x.dtype), _ffi.ptr(ws), nbytes)
+    return logprob, entropy, stats, top_lp, top_i
+
+
+def _grad_of(g, shape):
+    if g is None:
+        return None
+    assert g.shape == shape, f"a gradient must have its output's shape {tuple(shape)}"
+    return g.float().contiguous()
+
+
+def logprobs_bwd(x, targets, stats, entropy, top_i, dlogprob, dentropy, dtop):
+    rows, vocab = x.shape
+    dx = torch.empty((rows, vocab), dtype=x.dtype, device=x.device)
+    top_k = 0 if top_i is None else top_i.shape[1]
+    grads = [_grad_of(dlogprob, (rows,)), _grad_of(dentropy, (rows,)), _grad_of(dtop, (rows, top_k))]
+    if rows:
+        _ffi.launch(_ffi.lib().scree_token_logprobs_bwd, x, x.data_ptr(), x.stride(0),
+                    targets.data_ptr(), targets.element_size(), rows, vocab, top_k,
+                    stats.data_ptr(), entropy.data_ptr(), _ffi.ptr(top_i),
+                    *[_ffi.ptr(g) for g in grads], dx.data_ptr(), vocab,
+                    _ffi.dtype_code(x.dtype))
+    return dx
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k):
+        x, y = _rows_view(logits), targets.contiguous()
+        logprob, entropy, stats, top_lp, top_i = logprobs_fwd(x, y, top_k, True)
+        ctx.save_for_backward(x, y, stats, entropy, top_i)
+        ctx.set_materialize_grads(False)
+        if top_k == 0:
+            return logprob, entropy
+        ctx.mark_non_differentiable(top_i)
+        return logprob, entropy, top_lp, top_i
+
+    @staticmethod
+    def backward(ctx, dlogprob, dentropy, dtop=None, _=None):
+        if dlogprob is None and dentropy is None and dtop is None:
+            return None, None, None
+        return logprobs_bwd(*ctx.saved_tensors, dlogprob, dentropy, dtop), None, None
+
+
+def varlen_token_logprobs_hip(logits, targets, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``targets`` under packed ``logits`` ``(total, vocab)``.
+
+    ``targets`` are int32 or int64 ``(total,)`` on the same device.  A negative
+    target means the row has none: its log probability is 0 and sends no
+    gradient back.  A target past the vocabulary gives NaN (the host never
+    reads them).  ``top_k`` (0 to 64) asks for that many most likely tokens of
+    each row, in falling order, the lowest index first among equal logits.
+    Logits may be fp16, bf16 or fp32, their rows strided; the results are fp32.
+
+    A logit of -inf has probability zero.  A row with nothing but -inf, or
+    with a NaN or +inf, has NaN results, as ``torch.log_softmax``.
+    """
+    _check(logits, targets, top_k)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out = _TokenLogprobsFn.apply(logits, targets, top_k)
+        return TokenLogprobs(*out) if top_k else TokenLogprobs(*out, None, None)
+    logprob, entropy, _, top_lp, top_i = logprobs_fwd(_rows_view(logits), targets.contiguous(),
+                                                      top_k, False)
+    return TokenLogprobs(logprob, entropy, top_lp, top_i)
+
+
+def varlen_token_logprobs_hip_backward(logits, targets, dlogprob=None, dentropy=None,
+                                       dtop_logprob=None, top_k: int = 0):
+    """Gradient wrt ``logits`` of :func:`varlen_token_logprobs_hip` given the
+    gradients of its outputs (None for zero), the forward run again for its
+    statistics."""
+    _check(logits, targets, top_k)
+    x, y = _rows_view(logits.detach()), targets.contiguous()
+    _, entropy, stats, _, top_i = logprobs_fwd(x, y, top_k, True)
+    assert dtop_logprob is None or top_k, "dtop_logprob needs top_k"
+    return logprobs_bwd(x, y, stats, entropy, top_i, dlogprob, dentropy, dtop_logprob)
