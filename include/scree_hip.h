@@ -295,6 +295,56 @@ int scree_varlen_softmax_bwd(const void* y, const void* dy, void* dx, const int3
                              int batch, int64_t total_tokens, int64_t features, int dtype,
                              void* stream);
 
+/* --------------------------------------------------------- linear attention
+ * Per sequence and K/V head, with lam = exp(log_decay[kv_head]) (fp32, device):
+ *   S_t = lam S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t,
+ * S_{-1} the sequence's initial state, or zero; query head h reads K/V head
+ * h / (heads / kv_heads).  q is (total_tokens, heads, k_dim), k
+ * (total_tokens, kv_heads, k_dim), v (total_tokens, kv_heads, v_dim), o as q
+ * with v_dim, strided as the attention tensors; k_dim and v_dim are multiples
+ * of 8 from 8 to 256.  States are contiguous (batch, kv_heads, k_dim, v_dim)
+ * fp32.  16-bit products take their operands (scores, states, weighted values)
+ * rounded to that type; sums and states are fp32, and a state that is an
+ * output gets its operands in two (fp16) or three (bf16) terms.  The decay is
+ * a constant of the head: it has no gradient.  Offsets must ascend; others
+ * give unspecified values but never reach outside the tensors.  Rows of `o`
+ * past the last sequence are left as they were.  No counterpart in the
+ * reference. */
+
+/* Bytes of workspace for the forward (or the backward): the fp32 states
+ * between the segments that long sequences are walked in; 0 when no sequence
+ * can have two. */
+size_t scree_linear_attn_workspace_bytes(int batch, int64_t total_tokens, int heads, int kv_heads,
+                                         int k_dim, int v_dim, int backward);
+
+/* strides[8] = {q, k, v, o} x {row, head}, in elements.  initial_state and
+ * final_state may be NULL (zero; not wanted) and must not overlap. */
+int scree_linear_attn_fwd(const void* q, const void* k, const void* v, const float* log_decay,
+                          void* o, const float* initial_state, float* final_state,
+                          const int32_t* cu_seqlens, int batch, int64_t total_tokens, int heads,
+                          int kv_heads, int k_dim, int v_dim, const int64_t* strides, float scale,
+                          int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dq, dk, dv (and dinitial_state unless NULL) from dout, the final state's
+ * gradient (may be NULL: zero) and the forward's inputs; dk and dv sum over
+ * each group's query heads, without atomics.  Rows past the last sequence
+ * become zeros.  strides[14] = {dout, q, k, v, dq, dk, dv} x {row, head}. */
+int scree_linear_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                          const float* log_decay, void* dq, void* dk, void* dv,
+                          const float* initial_state, const float* dfinal_state,
+                          float* dinitial_state, const int32_t* cu_seqlens, int batch,
+                          int64_t total_tokens, int heads, int kv_heads, int k_dim, int v_dim,
+                          const int64_t* strides, float scale, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* One token for each of `rows` sequences: state_out = lam state + k v^T and
+ * o = scale * state_out^T q; state_out may be `state` (in place).
+ * strides[10] = {q, k, v, o} x {row, head}, {state row, state_out row}. */
+int scree_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay,
+                           void* o, const float* state, float* state_out, int64_t rows, int heads,
+                           int kv_heads, int k_dim, int v_dim, const int64_t* strides, float scale,
+                           int dtype, void* stream);
+
 /* ------------------------------------------------------ token log probabilities
  * Per row of `vocab` logits (rows `row_stride` elements apart, any alignment;
  * rows * ceil(vocab / 16384) at most 2^23) and its given token:

@@ -1,0 +1,938 @@
+// Varlen linear attention with a decay per head (gfx950): chunked walks for
+// packed sequences, forward and backward, and the recurrent single-token step.
+// No counterpart in the reference.
+//
+// Per sequence and K/V head with lam = exp(log_decay):
+//   S_t = lam S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,
+// S_{-1} the initial state or zero; query head h reads K/V head h / group.
+// With R_t = dL/dS_t = lam R_{t+1} + scale sum_group q_t do_t^T (the final
+// state's gradient joins at the last token),
+//   dq_t = scale S_t do_t,  dk_t = R_t v_t,  dv_t = R_t^T k_t,  dS_{-1} = lam R_0.
+// All four outputs are one walk over rows i (from the sequence's end for dk, dv),
+//   out_i = sum_{j <= i} lam^{i-j} (x_i . y_j) z_j + lam^{i+e} x_i A,
+// with (x, y, z) = (q, k, v), (do, v, k), (v, do, q), (k, q, do) and A the
+// state that came in: S, S^T, R^T, R.  e is 1 forward (the state is of the
+// token before) and 0 backward (the carried state is lam R of the row after,
+// or the final state's gradient itself).
+//
+// A workgroup walks a segment of a sequence in chunks of C rows with A in its
+// accumulators (fp32): per chunk P = X Y^T weighted by lam^{i-j} below the
+// diagonal, out = P Z + diag(lam^{i+e}) X A, then A = lam^n A + Y^T diag(..) Z.
+// Sequences longer than a segment are first reduced to their segments' own
+// states and these chained, so that segments walk side by side (a long
+// sequence alone fills the GPU).
+
+#include "common.h"
+
+namespace scree {
+namespace {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Frag { typedef typename VecT<T>::x8 t; };
+template <> struct Frag<float> { typedef f32x8 t; };
+
+// C(16x16, f32) += A(16x32) B(32x16): lane l holds A row l % 16 / B column
+// l % 16 with k = 8 (l / 16) .. + 7; C element i of lane l is row
+// 4 (l / 16) + i, column l % 16.  fp32 takes eight products of 4 k each.
+__device__ __forceinline__ void mma(f32x4& c, const f16x8& a, const f16x8& b) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x4& c, const bf16x8& a, const bf16x8& b) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x4& c, const f32x8& a, const f32x8& b) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+}
+
+// A ROWS x D tile in LDS, row-major, its 16-byte chunks permuted within a row
+// (chunk ^ swz(row)) so that reads of 16 rows at one chunk and transposed
+// reads of 4 rows spread over the banks.
+template <typename T, int D>
+struct Tile {
+  static constexpr int PER = 16 / sizeof(T);  // elements per chunk
+  static constexpr int CPR = D / PER;         // chunks per row
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (sizeof(T) == 4) {
+      const int s = (((row & 7) << 1) | ((row >> 3) & 1)) ^ (((row >> 4) & 1) << 3);
+      return CPR >= 16 ? s : (row >> 1) & 7;
+    } else {
+      return CPR >= 16 ? 4 * (row & 3) + ((row >> 2) & 3)
+           : CPR == 8  ? 4 * ((row >> 1) & 1) + ((row >> 2) & 3)
+                       : (row >> 2) & 3;
+    }
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return row * D + (chunk ^ swz(row)) * PER;
+  }
+  // columns [c0, c0 + 8) of a row, c0 a multiple of 8
+  static __device__ __forceinline__ typename Frag<T>::t row8(const T* t, int row, int c0) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(t + at(row, c0 / 4));
+      const float4 b = *reinterpret_cast<const float4*>(t + at(row, c0 / 4 + 1));
+      return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    } else {
+      return __builtin_bit_cast(typename Frag<T>::t, ld16(t + at(row, c0 / 8)));
+    }
+  }
+  // Transposed operand: lane l = 16 g + c gets column c0 + 8 (c / 4) + 4 half + c % 4
+  // of rows r0 + 8 g .. + 7 (c0 a multiple of 32).  Two halves make 32 columns
+  // of which an accumulator's lanes then hold 8 in a row.
+  // ds_read_b64_tr_b16 hands lane 16 g + c, slot j, element c % 4 of the 8
+  // bytes addressed by lane 16 g + 4 j + c / 4.
+  static __device__ __forceinline__ typename Frag<T>::t col8(const T* t, int r0, int c0, int half) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    if constexpr (sizeof(T) == 4) {
+      const int c = lane & 15, chunk = c0 / 4 + 2 * (c >> 2) + half;
+      f32x8 v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = t[at(r0 + 8 * g + j, chunk) + (c & 3)];
+      return v;
+    } else {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      typedef short s8 __attribute__((ext_vector_type(8)));
+      typedef __attribute__((address_space(3))) s4* lds_s4;
+      const int row = r0 + 8 * g + ((lane & 15) >> 2), chunk = c0 / 8 + (lane & 3);
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + at(row, chunk) + 4 * half));
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + at(row + 4, chunk) + 4 * half));
+      const s8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      return __builtin_bit_cast(typename Frag<T>::t, v);
+    }
+  }
+};
+
+// Rows of a tile on their way from memory to LDS, held in registers: the loads
+// of the next rows are issued before the products of the present ones.
+template <typename T, int D, int ROWS, int THREADS>
+struct Stage {
+  typedef Tile<T, D> L;
+  static constexpr int N = ROWS * L::CPR / THREADS;
+  static_assert(ROWS * L::CPR % THREADS == 0, "whole chunks per thread");
+  uint4 v[N];
+  // rows [0, n) of `base`, `step` elements apart (negative: backwards), columns
+  // below d; zeros elsewhere
+  __device__ __forceinline__ void load(const T* base, int64_t step, int n, int d) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int q = i * THREADS + threadIdx.x, r = q / L::CPR, c = q % L::CPR;
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < n && c * L::PER < d) v[i] = ld16(base + r * step + c * L::PER);
+    }
+  }
+  __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int q = i * THREADS + threadIdx.x;
+      st16(lds + L::at(q / L::CPR, q % L::CPR), v[i]);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::t to_frag(const float* f) {
+  if constexpr (sizeof(T) == 4) {
+    return f32x8{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+  } else {
+    return __builtin_bit_cast(typename Frag<T>::t, pack16<T>(f));
+  }
+}
+
+// ------------------------------------------------------------ the work items
+// Segment j of sequence b has slot cu[b] / M + b + j, M the segment length: a
+// sequence of L tokens has max(1, ceil(L / M)) segments, and slots of
+// different sequences never meet (floor(a) + ceil(l) <= floor(a + l) + 1), so
+// a workgroup finds its segment from the offsets alone.  Slots that no
+// segment has are skipped.  Offsets are clamped to [0, total].
+struct Segment {
+  int seq, index, count;  // the sequence, this segment's place in it, its number of segments
+  int64_t row0;           // first row
+  int rows;
+};
+__device__ __forceinline__ int64_t offset_at(const int32_t* cu, int i, int64_t total) {
+  return min<int64_t>(max<int64_t>(cu[i], 0), total);
+}
+__device__ __forceinline__ bool find_segment(const int32_t* __restrict__ cu, int batch, int64_t total,
+                                             int seg, int slot, Segment& s) {
+  int lo = 0, hi = batch - 1;  // the last sequence whose first slot is at most `slot`
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (offset_at(cu, mid, total) / seg + mid <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t a = offset_at(cu, lo, total), b = max(a, offset_at(cu, lo + 1, total));
+  s.seq = lo;
+  s.index = slot - (int)(a / seg) - lo;
+  s.count = max<int>(1, (int)((b - a + seg - 1) / seg));
+  if (s.index < 0 || s.index >= s.count) return false;
+  s.row0 = a + (int64_t)s.index * seg;
+  s.rows = (int)min<int64_t>(seg, b - s.row0);
+  return true;
+}
+
+struct Role {
+  const void *x, *y, *z;  // x null: the segment's state alone
+  void* out;
+  int64_t x_row, x_head, y_row, y_head, z_row, z_head, o_row, o_head;
+  const float* init;   // (batch, kv_heads, state): the state that comes in, may be null
+  float* last;         // (batch, kv_heads, state): the state that goes out, may be null
+  float* seg_state;    // (slots, kv_heads, state)
+  int64_t s_x, s_z;    // the state's strides along x's and z's axes
+  int heads;           // of x and out
+  int x_group;         // heads of x per K/V head
+  int y_group;         // heads of y and z per K/V head, summed
+  int dx, dz;
+  int reverse;
+  int zero_tail;       // rows past the last sequence become zeros (gradients)
+  float pscale, oscale;
+};
+constexpr int kMaxRoles = 3;
+struct WalkArgs {
+  Role role[kMaxRoles];
+  const int32_t* cu;
+  const float* log_decay;
+  int64_t total;
+  int batch, kv_heads, seg, slots;
+  int terms;  // 16-bit terms the update's operand is split into (1 to 3)
+};
+
+template <typename T, int DX> constexpr int chunk_rows() { return sizeof(T) == 4 && DX == 256 ? 32 : 64; }
+
+template <typename T, int DX, int NW, bool OUT>
+constexpr size_t walk_lds() {
+  constexpr int C = chunk_rows<T, DX>();
+  return sizeof(T) * (size_t)((OUT ? 2 : 1) * C * DX + C * 32 * NW + (OUT ? C * C : 0)) + 4 * (C + 4);
+}
+
+// NW waves; wave w owns columns [32 w, 32 w + 32) of z, out and the state.
+template <typename T, int DX, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW) void lin_walk_kernel(WalkArgs a) {
+  constexpr int C = chunk_rows<T, DX>();
+  constexpr int DZ = 32 * NW, THREADS = 64 * NW;
+  constexpr int ST = C / 16;  // strips of 16 rows
+  typedef Tile<T, DX> LX;
+  typedef Tile<T, DZ> LZ;
+  typedef Tile<T, C> LP;
+  typedef typename Frag<T>::t F;
+  extern __shared__ __align__(16) char lds_raw[];
+  T* ys = reinterpret_cast<T*>(lds_raw);
+  T* zs = ys + C * DX;
+  T* xs = zs + C * DZ;
+  T* ps = xs + (OUT ? C * DX : 0);
+  float* pow = reinterpret_cast<float*>(ps + (OUT ? C * C : 0));  // lam^0 .. lam^C
+
+  const Role& r = a.role[blockIdx.y];
+  const int slices = (r.dz + DZ - 1) / DZ;
+  const int heads = OUT ? r.heads : a.kv_heads;
+  int item = blockIdx.x;
+  const int slice = item % slices;
+  item /= slices;
+  const int head = item % heads, slot = item / heads;
+  if (slot >= a.slots) return;
+  const int kvh = OUT ? head / r.x_group : head;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int z0 = slice * DZ, zcols = min(DZ, r.dz - z0);
+
+  if constexpr (OUT) {
+    // rows behind the last sequence: the last slot's workgroups
+    if (r.zero_tail && slot == a.slots - 1) {
+      T* out = static_cast<T*>(r.out) + head * r.o_head + z0;
+      const int per = zcols / 8;
+      const int64_t tail = offset_at(a.cu, a.batch, a.total);
+      for (int64_t q = threadIdx.x; q < (a.total - tail) * per; q += THREADS) {
+        T* p = out + (tail + q / per) * r.o_row + (int)(q % per) * 8;
+        st16(p, make_uint4(0u, 0u, 0u, 0u));
+        if constexpr (sizeof(T) == 4) st16(p + 4, make_uint4(0u, 0u, 0u, 0u));
+      }
+    }
+  }
+  Segment sg;
+  if (!find_segment(a.cu, a.batch, a.total, a.seg, slot, sg)) return;
+  const int first = r.reverse ? sg.count - 1 : 0, final = sg.count - 1 - first;
+  // a segment whose state nobody reads
+  if (!OUT && (sg.index == final || sg.count == 1)) return;
+
+  const float g2 = a.log_decay[kvh] * 1.4426950408889634f;
+  // lam^n; lam^0 is 1 also for a decay of -inf
+  auto power = [&](int n) { return n == 0 ? 1.f : exp2f(g2 * (float)n); };
+  for (int n = threadIdx.x; n <= C; n += THREADS) pow[n] = power(n);
+  const int e = r.reverse ? 0 : 1;
+
+  // the state: element [2 s + t][u][i] is x-column 32 s + 8 g + 4 t + i,
+  // z-column 32 wave + 8 (c / 4) + 4 u + c % 4
+  f32x4 st[DX / 16][2];
+  const int64_t state_size = (int64_t)r.dx * r.dz;
+  const int scol = 32 * wave + 8 * (c >> 2) + (c & 3);  // + 4 u
+  const float* in = nullptr;
+  if constexpr (OUT) {
+    if (sg.index != first) in = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
+    else if (r.init) in = r.init + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
+  }
+#pragma unroll
+  for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dx = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + i, dz = scol + 4 * u;
+        st[m][u][i] = in && dx < r.dx && dz < zcols ? in[dx * r.s_x + (z0 + dz) * r.s_z] : 0.f;
+      }
+
+  // weights of P's tiles, lane (c, g) element i: row t = c, column s = 4 g + i,
+  // tiles d strips below the diagonal
+  float wd[ST][4];
+#pragma unroll
+  for (int d = 0; d < ST; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int lag = 16 * d + c - (4 * g + i);
+      wd[d][i] = lag >= 0 ? power(lag) * r.pscale : 0.f;
+    }
+
+  const int64_t row_first = r.reverse ? sg.row0 + sg.rows - 1 : sg.row0;
+  const int64_t dir = r.reverse ? -1 : 1;
+  const T* x = static_cast<const T*>(r.x) + (OUT ? row_first * r.x_row + head * r.x_head : 0);
+  const T* y = static_cast<const T*>(r.y) + row_first * r.y_row + (int64_t)kvh * r.y_group * r.y_head;
+  const T* z = static_cast<const T*>(r.z) + row_first * r.z_row + (int64_t)kvh * r.y_group * r.z_head + z0;
+  Stage<T, DX, C, THREADS> sx, sy;
+  Stage<T, DZ, C, THREADS> sz;
+  const int chunks = (sg.rows + C - 1) / C, steps = chunks * r.y_group;
+  auto fetch = [&](int step) {
+    const int ci = step / r.y_group, yg = step % r.y_group;
+    const int64_t i0 = (int64_t)ci * C * dir;
+    const int n = min(C, sg.rows - ci * C);
+    sy.load(y + i0 * r.y_row + yg * r.y_head, dir * r.y_row, n, r.dx);
+    sz.load(z + i0 * r.z_row + yg * r.z_head, dir * r.z_row, n, zcols);
+    if constexpr (OUT) {
+      if (yg == 0) sx.load(x + i0 * r.x_row, dir * r.x_row, n, r.dx);
+    }
+  };
+  f32x4 o[2][ST];
+  if (steps) fetch(0);
+  for (int step = 0; step < steps; ++step) {
+    const int ci = step / r.y_group, yg = step % r.y_group;
+    const int n = min(C, sg.rows - ci * C);
+    sy.store(ys);
+    sz.store(zs);
+    if constexpr (OUT) {
+      if (yg == 0) sx.store(xs);
+    }
+    __syncthreads();
+    if (step + 1 < steps) fetch(step + 1);
+
+    if constexpr (OUT) {
+      // P, a strip of 16 rows per wave and turn, rounded to T for the product with Z
+#pragma unroll
+      for (int s0 = 0; s0 < ST; s0 += NW) {
+        const int strip = s0 + wave;
+        if (NW > ST && strip >= ST) break;
+        F xf[DX / 32];
+#pragma unroll
+        for (int k = 0; k < DX / 32; ++k) xf[k] = LX::row8(xs, 16 * strip + c, 32 * k + 8 * g);
+#pragma unroll
+        for (int tile = 0; tile < ST; ++tile) {
+          if (tile > (strip | 1)) continue;  // the products read pairs of tiles
+          f32x4 p = {0.f, 0.f, 0.f, 0.f};
+          if (tile <= strip) {
+#pragma unroll
+            for (int k = 0; k < DX / 32; ++k) mma(p, LX::row8(ys, 16 * tile + c, 32 * k + 8 * g), xf[k]);
+            const int d = strip - tile;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float w = 0.f;  // wd[d][i] without a run-time register index
+#pragma unroll
+              for (int j = 0; j < ST; ++j) w = d == j ? wd[j][i] : w;
+              p[i] *= w;
+            }
+          }
+          const int col = 16 * tile + 4 * g;
+          T* dst = ps + LP::at(16 * strip + c, col / LP::PER) + col % LP::PER;
+          if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4*>(dst) = make_float4(p[0], p[1], p[2], p[3]);
+          else
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]));
+        }
+      }
+      // out^T = (X A)^T lam^{i+e}: the state's accumulators are its operand as they lie
+      if (yg == 0) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < DX / 32; ++k) {
+          F sf[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[i] = st[2 * k][u][i];
+              f[4 + i] = st[2 * k + 1][u][i];
+            }
+            sf[u] = to_frag<T>(f);
+          }
+#pragma unroll
+          for (int s = 0; s < ST; ++s) {
+            const F xf = LX::row8(xs, 16 * s + c, 32 * k + 8 * g);
+            mma(o[0][s], sf[0], xf);
+            mma(o[1][s], sf[1], xf);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+          const float w = pow[16 * s + c + e];
+          o[0][s] *= w;
+          o[1][s] *= w;
+        }
+      }
+      __syncthreads();
+    }
+    if (yg == 0) {
+      const float w = pow[n];
+#pragma unroll
+      for (int m = 0; m < DX / 16; ++m) {
+        st[m][0] *= w;
+        st[m][1] *= w;
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < C / 32; ++kk) {
+      const F zf[2] = {LZ::col8(zs, 32 * kk, 32 * wave, 0), LZ::col8(zs, 32 * kk, 32 * wave, 1)};
+      if constexpr (OUT) {
+#pragma unroll
+        for (int s = 2 * kk; s < ST; ++s) {
+          const F pf = LP::row8(ps, 16 * s + c, 32 * kk + 8 * g);
+          mma(o[0][s], zf[0], pf);
+          mma(o[1][s], zf[1], pf);
+        }
+      }
+      // Z weighted by lam^{n - e - i}, rounded to T (in `terms` terms, each the
+      // rounding of what the ones before leave)
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = pow[max(0, n - e - (32 * kk + 8 * g + j))] * r.pscale;
+      float rest[2][8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rest[u][j] = (float)zf[u][j] * w[j];
+      for (int t = 0; t < (sizeof(T) == 4 ? 1 : a.terms); ++t) {
+        F zw[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          zw[u] = to_frag<T>(rest[u]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) rest[u][j] -= (float)zw[u][j];
+        }
+#pragma unroll
+        for (int m = 0; m < DX / 16; ++m) {
+          const F yf = LX::col8(ys, 32 * kk, 32 * (m >> 1), m & 1);
+          mma(st[m][0], yf, zw[0]);
+          mma(st[m][1], yf, zw[1]);
+        }
+      }
+    }
+    if constexpr (OUT) {
+      if (yg == r.y_group - 1 && 32 * wave + 8 * g < zcols) {
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+          const int i = 16 * s + c;
+          if (i >= n) continue;
+          T* out = static_cast<T*>(r.out) + (row_first + dir * ((int64_t)ci * C + i)) * r.o_row +
+                   head * r.o_head + z0 + 32 * wave + 8 * g;
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            f[k] = o[0][s][k] * r.oscale;
+            f[4 + k] = o[1][s][k] * r.oscale;
+          }
+          st16(out, pack16<T>(f));
+          if constexpr (sizeof(T) == 4) st16(out + 4, pack16<T>(f + 4));
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  float* to = nullptr;
+  if constexpr (!OUT) {
+    to = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
+  } else {
+    if (r.last && sg.index == final && head % r.x_group == 0)
+      to = r.last + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
+  }
+  if (!to) return;
+#pragma unroll
+  for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dx = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + i, dz = scol + 4 * u;
+        if (dx < r.dx && dz < zcols) to[dx * r.s_x + (z0 + dz) * r.s_z] = st[m][u][i];
+      }
+}
+
+// The segments' own states become the states that come into them: along each
+// sequence, in = lam^rows in + own.  A thread per four elements.
+constexpr int kChainThreads = 256;
+__global__ __launch_bounds__(kChainThreads) void lin_chain_kernel(WalkArgs a) {
+  const Role& r = a.role[blockIdx.y];
+  const int64_t state = (int64_t)r.dx * r.dz;
+  const int per = (int)((state / 4 + kChainThreads - 1) / kChainThreads);
+  int item = blockIdx.x;
+  const int64_t q = (int64_t)(item % per) * kChainThreads + threadIdx.x;
+  item /= per;
+  const int kvh = item % a.kv_heads, seq = item / a.kv_heads;
+  const int64_t s0 = offset_at(a.cu, seq, a.total), s1 = max(s0, offset_at(a.cu, seq + 1, a.total));
+  const int count = (int)((s1 - s0 + a.seg - 1) / a.seg);
+  if (count < 2 || q * 4 >= state) return;
+  const int slot0 = (int)(s0 / a.seg) + seq;
+  const float g2 = a.log_decay[kvh] * 1.4426950408889634f;
+  float4 cur = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (r.init) cur = *reinterpret_cast<const float4*>(r.init + ((int64_t)seq * a.kv_heads + kvh) * state + 4 * q);
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < count; j0 += U) {
+    float4 own[U];
+    float4* at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = r.reverse ? count - 1 - (j0 + u) : j0 + u;
+      at[u] = reinterpret_cast<float4*>(r.seg_state + ((int64_t)(slot0 + j) * a.kv_heads + kvh) * state) + q;
+      // the last segment has no state of its own
+      if (j0 + u < count - 1) own[u] = *at[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j0 + u >= count) continue;
+      *at[u] = cur;
+      if (j0 + u >= count - 1) continue;
+      const int j = r.reverse ? count - 1 - (j0 + u) : j0 + u;
+      const int rows = (int)min<int64_t>(a.seg, s1 - s0 - (int64_t)j * a.seg);
+      const float w = exp2f(g2 * (float)rows);
+      cur.x = fmaf(w, cur.x, own[u].x);
+      cur.y = fmaf(w, cur.y, own[u].y);
+      cur.z = fmaf(w, cur.z, own[u].z);
+      cur.w = fmaf(w, cur.w, own[u].w);
+    }
+  }
+}
+
+// ------------------------------------------------------------- single tokens
+// S = lam S + k v^T and o = scale S^T q for one token per row of a batch: a
+// workgroup per row, K/V head and 32 columns of the state, which it reads and
+// writes once (8 lanes of 4 columns by 32 rows; a thread holds its rows' 4
+// columns while the group's query heads read them).
+constexpr int kStepThreads = 256;
+struct StepArgs {
+  const void *q, *k, *v;
+  void* out;
+  const float* log_decay;
+  const float* state;
+  float* state_out;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, s_row, so_row;
+  int kv_heads, group, dk, dv;
+  float scale;
+};
+template <typename T, int ROWS>  // ROWS * 32 >= dk
+__global__ __launch_bounds__(kStepThreads) void lin_step_kernel(StepArgs a) {
+  __shared__ float qs[ROWS * 32];
+  __shared__ float4 part[kStepThreads / 64][8];
+  const int tiles = (a.dv + 31) / 32;
+  int item = blockIdx.x;
+  const int tile = item % tiles;
+  item /= tiles;
+  const int kvh = item % a.kv_heads;
+  const int64_t row = item / a.kv_heads;
+  const int cl = threadIdx.x & 7, rl = threadIdx.x >> 3;
+  const int col = 32 * tile + 4 * cl;
+  const bool live = col < a.dv;
+  const float lam = expf(a.log_decay[kvh]);
+  const T* k = static_cast<const T*>(a.k) + row * a.k_row + kvh * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + row * a.v_row + kvh * a.v_head;
+  const int64_t base = (int64_t)kvh * a.dk * a.dv + col;
+  const float* s = a.state + row * a.s_row + base;
+  float* so = a.state_out + row * a.so_row + base;
+  float4 st[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int d = 32 * i + rl;
+    st[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live && d < a.dk) st[i] = *reinterpret_cast<const float4*>(s + (int64_t)d * a.dv);
+  }
+  float vv[4] = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = to_f32(v[col + j]);
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int d = 32 * i + rl;
+    if (!live || d >= a.dk) continue;
+    const float kd = to_f32(k[d]);
+    st[i].x = fmaf(lam, st[i].x, kd * vv[0]);
+    st[i].y = fmaf(lam, st[i].y, kd * vv[1]);
+    st[i].z = fmaf(lam, st[i].z, kd * vv[2]);
+    st[i].w = fmaf(lam, st[i].w, kd * vv[3]);
+    *reinterpret_cast<float4*>(so + (int64_t)d * a.dv) = st[i];
+  }
+  for (int h = 0; h < a.group; ++h) {
+    const int head = kvh * a.group + h;
+    const T* q = static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head;
+    for (int d = threadIdx.x; d < ROWS * 32; d += kStepThreads) qs[d] = d < a.dk ? to_f32(q[d]) : 0.f;
+    __syncthreads();
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const float qd = qs[32 * i + rl];
+      acc.x = fmaf(qd, st[i].x, acc.x);
+      acc.y = fmaf(qd, st[i].y, acc.y);
+      acc.z = fmaf(qd, st[i].z, acc.z);
+      acc.w = fmaf(qd, st[i].w, acc.w);
+    }
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) {
+      acc.x += __shfl_xor(acc.x, o);
+      acc.y += __shfl_xor(acc.y, o);
+      acc.z += __shfl_xor(acc.z, o);
+      acc.w += __shfl_xor(acc.w, o);
+    }
+    if ((threadIdx.x & 63) < 8) part[threadIdx.x >> 6][cl] = acc;
+    __syncthreads();
+    if (threadIdx.x < 8 && live) {
+      float4 t = part[0][cl];
+#pragma unroll
+      for (int w = 1; w < kStepThreads / 64; ++w) {
+        t.x += part[w][cl].x;
+        t.y += part[w][cl].y;
+        t.z += part[w][cl].z;
+        t.w += part[w][cl].w;
+      }
+      T* o = static_cast<T*>(a.out) + row * a.o_row + head * a.o_head + col;
+      o[0] = from_f32<T>(t.x * a.scale);
+      o[1] = from_f32<T>(t.y * a.scale);
+      o[2] = from_f32<T>(t.z * a.scale);
+      o[3] = from_f32<T>(t.w * a.scale);
+    }
+  }
+}
+
+// ------------------------------------------------------------------- host
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Tokens per segment: enough segments to give the GPU kLinFill workgroups, of
+// at least kLinMinSeg tokens (their states cost as much traffic as that many
+// tokens) and at most kLinMaxSeg (the longest walk).
+constexpr int64_t kLinFill = 1024;
+constexpr int kLinMinSeg = 256, kLinMaxSeg = 2048;
+
+inline int segment_tokens(int64_t total, int heads) {
+  int64_t m = (total * heads / kLinFill + 63) / 64 * 64;
+  if (m < kLinMinSeg) m = kLinMinSeg;
+  if (m > kLinMaxSeg) m = kLinMaxSeg;
+  return (int)m;
+}
+inline int64_t slot_count(int64_t total, int batch, int seg) { return total / seg + batch; }
+
+struct Shape {
+  int batch, heads, kv_heads, dk, dv, dtype;
+  int64_t total;
+};
+
+int check_shape(const char* fn, const Shape& s) {
+  if (s.batch < 1) return set_error(SCREE_ERR_UNSUPPORTED, "%s: batch must be at least 1, got %d", fn, s.batch);
+  if (s.total < 0 || s.total > ((int64_t)1 << 30))
+    return set_error(SCREE_ERR_INVALID, "%s: total_tokens %lld out of range", fn, (long long)s.total);
+  if (s.heads < 1 || s.heads > 4096 || s.kv_heads < 1 || s.heads % s.kv_heads)
+    return set_error(SCREE_ERR_INVALID, "%s: heads %d (at most 4096) must be a multiple of kv_heads %d", fn,
+                     s.heads, s.kv_heads);
+  for (int d : {s.dk, s.dv})
+    if (d < 8 || d > 256 || d % 8)
+      return set_error(SCREE_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (multiples of 8 up to 256)", fn, d);
+  if (s.dtype != SCREE_DTYPE_F16 && s.dtype != SCREE_DTYPE_BF16 && s.dtype != SCREE_DTYPE_F32)
+    return set_error(SCREE_ERR_UNSUPPORTED, "%s: dtype code %d unsupported (fp16, bf16, fp32)", fn, s.dtype);
+  return SCREE_OK;
+}
+
+struct Arg {
+  const char* name;
+  const void* p;
+  const int64_t* st;
+  int dim;
+};
+int check_args(const char* fn, const Arg* args, int n, int64_t rows) {
+  for (int i = 0; i < n; ++i) {
+    const Arg& t = args[i];
+    if (!t.p) return set_error(SCREE_ERR_INVALID, "%s: %s is null", fn, t.name);
+    if (!aligned16(t.p)) return set_error(SCREE_ERR_INVALID, "%s: %s is not 16-byte aligned", fn, t.name);
+    for (int k = 0; k < 2; ++k)
+      if (t.st[k] % 8 || t.st[k] < 0 || t.st[k] >= ((int64_t)1 << 24))
+        return set_error(SCREE_ERR_INVALID,
+                         "%s: %s strides (%lld, %lld) must be multiples of 8 elements in [0, 2^24)", fn, t.name,
+                         (long long)t.st[0], (long long)t.st[1]);
+    if (rows > 1 && t.st[0] < t.dim)
+      return set_error(SCREE_ERR_INVALID, "%s: %s row stride %lld overlaps rows", fn, t.name, (long long)t.st[0]);
+  }
+  return SCREE_OK;
+}
+int check_states(const char* fn, const void* const* p, int n) {
+  for (int i = 0; i < n; ++i)
+    if (p[i] && !aligned16(p[i])) return set_error(SCREE_ERR_INVALID, "%s: a state is not 16-byte aligned", fn);
+  return SCREE_OK;
+}
+
+// Bytes of one set of segment states (0: no sequence can have two segments).
+size_t states_bytes(const Shape& s) {
+  const int seg = segment_tokens(s.total, s.heads);
+  if (s.total <= seg) return 0;
+  return (size_t)slot_count(s.total, s.batch, seg) * s.kv_heads * s.dk * s.dv * sizeof(float);
+}
+
+template <typename T, int DX, int NW, bool OUT>
+int launch_walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
+  int64_t items = 0;
+  for (int i = 0; i < roles; ++i) {
+    const Role& r = a.role[i];
+    const int64_t n = (int64_t)a.slots * (OUT ? r.heads : a.kv_heads) * ((r.dz + 32 * NW - 1) / (32 * NW));
+    if (n > items) items = n;
+  }
+  if (items * 64 * NW > 0xffffffffll)
+    return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
+  constexpr size_t lds = walk_lds<T, DX, NW, OUT>();
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  auto kernel = lin_walk_kernel<T, DX, NW, OUT>;
+  if (lds > 64 * 1024) {
+    const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (rc != hipSuccess) return set_error(SCREE_ERR_HIP, "%s: %s", fn, hipGetErrorString(rc));
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)items, roles), dim3(64 * NW), lds, stream, a);
+  return check_launch(fn);
+}
+template <typename T, bool OUT, int DX>
+int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
+  const int dz = a.role[0].dz;
+  if (dz <= 32) return launch_walk<T, DX, 1, OUT>(fn, a, roles, stream);
+  if (dz <= 64) return launch_walk<T, DX, 2, OUT>(fn, a, roles, stream);
+  return launch_walk<T, DX, 4, OUT>(fn, a, roles, stream);
+}
+// One launch for `roles` walks of equal dims.
+template <typename T, bool OUT>
+int walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
+  const int dx = a.role[0].dx;
+  if (dx <= 32) return walk_z<T, OUT, 32>(fn, a, roles, stream);
+  if (dx <= 64) return walk_z<T, OUT, 64>(fn, a, roles, stream);
+  if (dx <= 128) return walk_z<T, OUT, 128>(fn, a, roles, stream);
+  return walk_z<T, OUT, 256>(fn, a, roles, stream);
+}
+template <typename T>
+int segment_states(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
+  if (int rc = walk<T, false>(fn, a, roles, stream)) return rc;
+  const int64_t state = (int64_t)a.role[0].dx * a.role[0].dz;
+  const int64_t per = (state / 4 + kChainThreads - 1) / kChainThreads;
+  const int64_t items = per * a.kv_heads * a.batch;
+  if (items * kChainThreads > 0xffffffffll)
+    return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
+  hipLaunchKernelGGL(lin_chain_kernel, dim3((unsigned)items, roles), dim3(kChainThreads), 0, stream, a);
+  return check_launch(fn);
+}
+
+WalkArgs common_args(const Shape& s, const int32_t* cu, const float* log_decay, int terms) {
+  WalkArgs a = {};
+  a.cu = cu;
+  a.log_decay = log_decay;
+  a.total = s.total;
+  a.batch = s.batch;
+  a.kv_heads = s.kv_heads;
+  a.seg = segment_tokens(s.total, s.heads);
+  a.slots = (int)slot_count(s.total, s.batch, a.seg);
+  a.terms = terms;
+  return a;
+}
+
+// 16-bit terms of the weighted operand in the states' updates: one where a
+// state only feeds outputs of the same 16 bits, enough for fp32 where it is
+// an output itself.
+int update_terms(int dtype, bool state_out) {
+  if (!state_out) return 1;
+  return dtype == SCREE_DTYPE_BF16 ? 3 : 2;
+}
+
+template <typename T>
+int run_fwd(const char* fn, const Shape& s, const void* q, const void* k, const void* v, void* o,
+            const float* log_decay, const int32_t* cu, const float* init, float* last,
+            const int64_t* st, float scale, void* workspace, hipStream_t stream) {
+  WalkArgs a = common_args(s, cu, log_decay, update_terms(s.dtype, last != nullptr));
+  const int group = s.heads / s.kv_heads;
+  a.role[0] = {q, k, v, o, st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7],
+               init, last, static_cast<float*>(workspace), s.dv, 1,
+               s.heads, group, 1, s.dk, s.dv, 0, 0, 1.f, scale};
+  if (s.total > a.seg)
+    if (int rc = segment_states<T>(fn, a, 1, stream)) return rc;
+  return walk<T, true>(fn, a, 1, stream);
+}
+
+template <typename T>
+int run_bwd(const char* fn, const Shape& s, const void* dout, const void* q, const void* k, const void* v,
+            void* dq, void* dk, void* dv, const float* log_decay, const int32_t* cu, const float* init,
+            const float* dlast, float* dinit, const int64_t* st, float scale, void* workspace,
+            hipStream_t stream) {
+  WalkArgs a = common_args(s, cu, log_decay, update_terms(s.dtype, dinit != nullptr));
+  const int group = s.heads / s.kv_heads;
+  float* seg_s = static_cast<float*>(workspace);
+  float* seg_r = seg_s + states_bytes(s) / sizeof(float);
+  const int64_t *sdo = st, *sq = st + 2, *sk = st + 4, *sv = st + 6, *sdq = st + 8, *sdk = st + 10, *sdv = st + 12;
+  if (s.total > a.seg) {
+    // S forward from (k, v), R backward from (q, dout), both dk x dv
+    a.role[0] = {nullptr, k, v, nullptr, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0,
+                 init, nullptr, seg_s, s.dv, 1, s.heads, group, 1, s.dk, s.dv, 0, 0, 1.f, 1.f};
+    a.role[1] = {nullptr, q, dout, nullptr, 0, 0, sq[0], sq[1], sdo[0], sdo[1], 0, 0,
+                 dlast, nullptr, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 0, scale, 1.f};
+    if (int rc = segment_states<T>(fn, a, 2, stream)) return rc;
+  }
+  const Role rdq = {dout, v, k, dq, sdo[0], sdo[1], sv[0], sv[1], sk[0], sk[1], sdq[0], sdq[1],
+                    init, nullptr, seg_s, 1, s.dv, s.heads, group, 1, s.dv, s.dk, 0, 1, 1.f, scale};
+  const Role rdk = {v, dout, q, dk, sv[0], sv[1], sdo[0], sdo[1], sq[0], sq[1], sdk[0], sdk[1],
+                    dlast, nullptr, seg_r, 1, s.dv, s.kv_heads, 1, group, s.dv, s.dk, 1, 1, scale, 1.f};
+  const Role rdv = {k, q, dout, dv, sk[0], sk[1], sq[0], sq[1], sdo[0], sdo[1], sdv[0], sdv[1],
+                    dlast, dinit, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 1, scale, 1.f};
+  a.role[0] = rdk;
+  a.role[1] = rdq;
+  a.role[2] = rdv;
+  if (s.dk == s.dv) return walk<T, true>(fn, a, 3, stream);
+  if (int rc = walk<T, true>(fn, a, 2, stream)) return rc;
+  a.role[0] = rdv;
+  return walk<T, true>(fn, a, 1, stream);
+}
+
+template <typename T>
+int run_step(const char* fn, const StepArgs& a, int64_t rows, hipStream_t stream) {
+  const int64_t items = rows * a.kv_heads * ((a.dv + 31) / 32);
+  if (items * kStepThreads > 0xffffffffll)
+    return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
+  const dim3 grid((unsigned)items);
+  const int need = (a.dk + 31) / 32;
+  if (need <= 1) hipLaunchKernelGGL((lin_step_kernel<T, 1>), grid, dim3(kStepThreads), 0, stream, a);
+  else if (need <= 2) hipLaunchKernelGGL((lin_step_kernel<T, 2>), grid, dim3(kStepThreads), 0, stream, a);
+  else if (need <= 4) hipLaunchKernelGGL((lin_step_kernel<T, 4>), grid, dim3(kStepThreads), 0, stream, a);
+  else hipLaunchKernelGGL((lin_step_kernel<T, 8>), grid, dim3(kStepThreads), 0, stream, a);
+  return check_launch(fn);
+}
+
+}  // namespace
+}  // namespace scree
+
+using namespace scree;
+
+extern "C" size_t scree_linear_attn_workspace_bytes(int batch, int64_t total_tokens, int heads,
+                                                    int kv_heads, int k_dim, int v_dim, int backward) {
+  const Shape s = {batch, heads, kv_heads, k_dim, v_dim, SCREE_DTYPE_F32, total_tokens};
+  if (check_shape("scree_linear_attn_workspace_bytes", s)) return 0;
+  return states_bytes(s) * (backward ? 2 : 1);
+}
+
+extern "C" int scree_linear_attn_fwd(const void* q, const void* k, const void* v, const float* log_decay,
+                                     void* o, const float* initial_state, float* final_state,
+                                     const int32_t* cu_seqlens, int batch, int64_t total_tokens,
+                                     int heads, int kv_heads, int k_dim, int v_dim,
+                                     const int64_t* strides, float scale, int dtype, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  const char* fn = "scree_linear_attn_fwd";
+  const Shape s = {batch, heads, kv_heads, k_dim, v_dim, dtype, total_tokens};
+  if (int rc = check_shape(fn, s)) return rc;
+  if (!cu_seqlens || !log_decay || !strides)
+    return set_error(SCREE_ERR_INVALID, "%s: cu_seqlens, log_decay or strides is null", fn);
+  const void* states[] = {initial_state, final_state};
+  if (int rc = check_states(fn, states, 2)) return rc;
+  if (total_tokens) {
+    const Arg args[] = {{"q", q, strides, k_dim}, {"k", k, strides + 2, k_dim},
+                        {"v", v, strides + 4, v_dim}, {"o", o, strides + 6, v_dim}};
+    if (int rc = check_args(fn, args, 4, total_tokens)) return rc;
+  } else if (!final_state) {
+    return SCREE_OK;
+  }
+  const size_t need = states_bytes(s);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(SCREE_ERR_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", fn, need,
+                     workspace ? workspace_bytes : (size_t)0);
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case SCREE_DTYPE_F32:
+      return run_fwd<float>(fn, s, q, k, v, o, log_decay, cu_seqlens, initial_state, final_state, strides, scale, workspace, hs);
+    case SCREE_DTYPE_F16:
+      return run_fwd<f16>(fn, s, q, k, v, o, log_decay, cu_seqlens, initial_state, final_state, strides, scale, workspace, hs);
+    default:
+      return run_fwd<bf16>(fn, s, q, k, v, o, log_decay, cu_seqlens, initial_state, final_state, strides, scale, workspace, hs);
+  }
+}
+
+extern "C" int scree_linear_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                                     const float* log_decay, void* dq, void* dk, void* dv,
+                                     const float* initial_state, const float* dfinal_state,
+                                     float* dinitial_state, const int32_t* cu_seqlens, int batch,
+                                     int64_t total_tokens, int heads, int kv_heads, int k_dim,
+                                     int v_dim, const int64_t* strides, float scale, int dtype,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "scree_linear_attn_bwd";
+  const Shape s = {batch, heads, kv_heads, k_dim, v_dim, dtype, total_tokens};
+  if (int rc = check_shape(fn, s)) return rc;
+  if (!cu_seqlens || !log_decay || !strides)
+    return set_error(SCREE_ERR_INVALID, "%s: cu_seqlens, log_decay or strides is null", fn);
+  const void* states[] = {initial_state, dfinal_state, dinitial_state};
+  if (int rc = check_states(fn, states, 3)) return rc;
+  if (total_tokens) {
+    const Arg args[] = {{"dout", dout, strides, v_dim}, {"q", q, strides + 2, k_dim},
+                        {"k", k, strides + 4, k_dim}, {"v", v, strides + 6, v_dim},
+                        {"dq", dq, strides + 8, k_dim}, {"dk", dk, strides + 10, k_dim},
+                        {"dv", dv, strides + 12, v_dim}};
+    if (int rc = check_args(fn, args, 7, total_tokens)) return rc;
+  } else if (!dinitial_state) {
+    return SCREE_OK;
+  }
+  const size_t need = 2 * states_bytes(s);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(SCREE_ERR_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", fn, need,
+                     workspace ? workspace_bytes : (size_t)0);
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case SCREE_DTYPE_F32:
+      return run_bwd<float>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, strides, scale, workspace, hs);
+    case SCREE_DTYPE_F16:
+      return run_bwd<f16>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, strides, scale, workspace, hs);
+    default:
+      return run_bwd<bf16>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, strides, scale, workspace, hs);
+  }
+}
+
+extern "C" int scree_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay,
+                                      void* o, const float* state, float* state_out, int64_t rows,
+                                      int heads, int kv_heads, int k_dim, int v_dim,
+                                      const int64_t* strides, float scale, int dtype, void* stream) {
+  const char* fn = "scree_linear_attn_step";
+  const Shape s = {1, heads, kv_heads, k_dim, v_dim, dtype, rows};
+  if (int rc = check_shape(fn, s)) return rc;
+  if (rows == 0) return SCREE_OK;
+  if (!log_decay || !strides || !state || !state_out)
+    return set_error(SCREE_ERR_INVALID, "%s: log_decay, strides or a state is null", fn);
+  const void* states[] = {state, state_out};
+  if (int rc = check_states(fn, states, 2)) return rc;
+  const Arg args[] = {{"q", q, strides, k_dim}, {"k", k, strides + 2, k_dim},
+                      {"v", v, strides + 4, v_dim}, {"o", o, strides + 6, v_dim}};
+  if (int rc = check_args(fn, args, 4, rows)) return rc;
+  const int64_t size = (int64_t)kv_heads * k_dim * v_dim;
+  for (int i = 8; i < 10; ++i)
+    if (strides[i] % 4 || (rows > 1 && strides[i] < size))
+      return set_error(SCREE_ERR_INVALID, "%s: state row stride %lld must be a multiple of 4 of at least %lld", fn,
+                       (long long)strides[i], (long long)size);
+  const StepArgs a = {q, k, v, o, log_decay, state, state_out, strides[0], strides[1], strides[2], strides[3],
+                      strides[4], strides[5], strides[6], strides[7], strides[8], strides[9],
+                      kv_heads, heads / kv_heads, k_dim, v_dim, scale};
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case SCREE_DTYPE_F32: return run_step<float>(fn, a, rows, hs);
+    case SCREE_DTYPE_F16: return run_step<f16>(fn, a, rows, hs);
+    default: return run_step<bf16>(fn, a, rows, hs);
+  }
+}

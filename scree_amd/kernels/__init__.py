@@ -113,6 +113,37 @@ def varlen_softmax(arr: Array) -> Array:
     return Array._trusted(varlen_softmax_hip(arr.values, arr.offsets), arr.offsets, 0)
 
 
+def varlen_linear_attention(q: Array, k: Array, v: Array, log_decay, scale=None, initial_state=None,
+                            return_state: bool = False):
+    """Per-sequence linear attention with a decay per head, of packed arrays.
+
+    The causal recurrence ``S_t = exp(log_decay) S_{t-1} + k_t v_t^T``,
+    ``o_t = scale q_t S_t`` on ``(total, heads, dim)`` arrays; see
+    :func:`scree_amd.kernels.hip.varlen_linear_attention_hip` for the
+    arguments.  Offsets must be identical for q, k, v (``ValueError``
+    otherwise).  Returns the output Array, or ``(output, state)`` with
+    ``return_state``, the states going on to the next call or to
+    :func:`scree_amd.kernels.hip.linear_attention_step_hip`.  No counterpart
+    in the reference.
+    """
+    import torch
+
+    from .hip import varlen_linear_attention_hip
+
+    for a in (q, k, v):
+        _require_device(a.values, "varlen_linear_attention")
+        if a.ragged_dim != 0:
+            raise NotImplementedError("varlen_linear_attention supports ragged_dim=0 only")
+    if not (q.offsets is k.offsets and q.offsets is v.offsets):
+        if not (torch.equal(q.offsets, k.offsets) and torch.equal(q.offsets, v.offsets)):
+            raise ValueError("q, k, v must have identical offsets")
+    out = varlen_linear_attention_hip(q.values, k.values, v.values, log_decay, q.offsets, scale,
+                                      initial_state, return_state)
+    if return_state:
+        return Array._trusted(out[0], q.offsets, 0), out[1]
+    return Array._trusted(out, q.offsets, 0)
+
+
 def varlen_token_logprobs(logits: Array, targets, top_k: int = 0):
     """Log probabilities of given tokens under packed ``(total, vocab)`` logits.
 
@@ -137,5 +168,5 @@ def varlen_token_logprobs(logits: Array, targets, top_k: int = 0):
     return TokenLogprobs(*[None if t is None else Array._trusted(t, logits.offsets, 0) for t in out])
 
 
-__all__ = ["varlen_add_rmsnorm", "varlen_attention", "varlen_layernorm", "varlen_rmsnorm",
-           "varlen_softmax", "varlen_token_logprobs"]
+__all__ = ["varlen_add_rmsnorm", "varlen_attention", "varlen_layernorm",
+           "varlen_linear_attention", "varlen_rmsnorm", "varlen_softmax", "varlen_token_logprobs"]

@@ -22,6 +22,11 @@ from .attention import (
     varlen_attention_hip,
     varlen_attention_hip_backward,
 )
+from .linear_attention import (
+    linear_attention_step_hip,
+    varlen_linear_attention_hip,
+    varlen_linear_attention_hip_backward,
+)
 from .logprobs import (
     TokenLogprobs,
     varlen_token_logprobs_hip,
@@ -58,6 +63,7 @@ __all__ = [
     "TokenLogprobs",
     "VarlenAttentionHip",
     "attention_schedule",
+    "linear_attention_step_hip",
     "needs_schedule",
     "prepare_workspace",
     "schedule_items",
@@ -69,6 +75,8 @@ __all__ = [
     "varlen_layernorm_hip",
     "varlen_layernorm_hip_autograd",
     "varlen_layernorm_hip_backward",
+    "varlen_linear_attention_hip",
+    "varlen_linear_attention_hip_backward",
     "varlen_rmsnorm_hip",
     "varlen_rmsnorm_hip_autograd",
     "varlen_rmsnorm_hip_backward",
