@@ -46,61 +46,101 @@ __device__ __forceinline__ void mma(f32x4& c, const f32x8& a, const f32x8& b) {
   for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
 }
 
-// A ROWS x D tile in LDS, row-major, its 16-byte chunks permuted within a row
-// (chunk ^ swz(row)) so that reads of 16 rows at one chunk and transposed
-// reads of 4 rows spread over the banks.
+// A tile of D columns in LDS, row-major, rows 16 bytes apart beyond their
+// length: 16 rows at one 16-byte chunk then cover the 256 bytes the LDS serves
+// a pass, and every address is a lane's own base plus a constant.
+//
+// Operands that run along the rows (transposed ones, with k = 32 rows of the
+// tile) hold in slot j of lane group g row tok(g, j), an order in which their
+// reads spread over the banks as well: 16-bit reads take 4 rows x 32 bytes per
+// lane group, every other row of 8 (16-byte steps would meet halfway); fp32
+// reads 64 bytes of rows 4 apart.  P's columns, which meet them, follow.
 template <typename T, int D>
 struct Tile {
   static constexpr int PER = 16 / sizeof(T);  // elements per chunk
   static constexpr int CPR = D / PER;         // chunks per row
-  static __device__ __forceinline__ int swz(int row) {
-    if constexpr (sizeof(T) == 4) {
-      const int s = (((row & 7) << 1) | ((row >> 3) & 1)) ^ (((row >> 4) & 1) << 3);
-      return CPR >= 16 ? s : (row >> 1) & 7;
-    } else {
-      return CPR >= 16 ? 4 * (row & 3) + ((row >> 2) & 3)
-           : CPR == 8  ? 4 * ((row >> 1) & 1) + ((row >> 2) & 3)
-                       : (row >> 2) & 3;
-    }
+  static constexpr int PITCH = D + PER;       // elements from row to row
+  static __device__ __forceinline__ constexpr int tok(int j) {  // without the group's part
+    return sizeof(T) == 4 ? (j & 3) + 16 * (j >> 2) : j < 4 ? 2 * j : 2 * j - 7;
   }
-  static __device__ __forceinline__ int at(int row, int chunk) {
-    return row * D + (chunk ^ swz(row)) * PER;
+  static constexpr int TOK_G = sizeof(T) == 4 ? 4 : 8;  // the group's part: TOK_G g
+
+  // This lane's place in the reads below, to which (row, col) constants add.
+  static __device__ __forceinline__ const T* row8_base(const T* t, int c, int g) { return t + c * PITCH + 8 * g; }
+  static __device__ __forceinline__ const T* row44_base(const T* t, int c, int g) { return t + c * PITCH + 4 * g; }
+  static __device__ __forceinline__ const T* col8_base(const T* t, int c, int g) {
+    if constexpr (sizeof(T) == 4) return t + TOK_G * g * PITCH + c;
+    else return t + (TOK_G * g + 2 * (c >> 2)) * PITCH + 4 * (c & 3);
   }
-  // columns [c0, c0 + 8) of a row, c0 a multiple of 8
-  static __device__ __forceinline__ typename Frag<T>::t row8(const T* t, int row, int c0) {
+  // columns col + 8 g .. + 7 of row + c
+  static __device__ __forceinline__ typename Frag<T>::t row8(const T* base, int row, int col) {
+    const T* p = base + row * PITCH + col;
     if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(t + at(row, c0 / 4));
-      const float4 b = *reinterpret_cast<const float4*>(t + at(row, c0 / 4 + 1));
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
       return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     } else {
-      return __builtin_bit_cast(typename Frag<T>::t, ld16(t + at(row, c0 / 8)));
+      return __builtin_bit_cast(typename Frag<T>::t, ld16(p));
     }
   }
-  // Transposed operand: lane l = 16 g + c gets column c0 + 8 (c / 4) + 4 half + c % 4
-  // of rows r0 + 8 g .. + 7 (c0 a multiple of 32).  Two halves make 32 columns
-  // of which an accumulator's lanes then hold 8 in a row.
-  // ds_read_b64_tr_b16 hands lane 16 g + c, slot j, element c % 4 of the 8
-  // bytes addressed by lane 16 g + 4 j + c / 4.
-  static __device__ __forceinline__ typename Frag<T>::t col8(const T* t, int r0, int c0, int half) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+  // columns col + 4 g .. + 3 and col + 16 + 4 g .. + 3 of row + c: the order in
+  // which two accumulators hold 32 rows
+  static __device__ __forceinline__ typename Frag<T>::t row44(const T* base, int row, int col) {
+    const T* p = base + row * PITCH + col;
     if constexpr (sizeof(T) == 4) {
-      const int c = lane & 15, chunk = c0 / 4 + 2 * (c >> 2) + half;
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
+      return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    } else {
+      const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 16);
+      return __builtin_bit_cast(typename Frag<T>::t, make_uint4(a.x, a.y, b.x, b.y));
+    }
+  }
+  // column col + c of rows row + TOK_G g + tok(j).  ds_read_b64_tr_b16 hands
+  // lane 16 g + c, slot j, element c % 4 of the 8 bytes addressed by lane
+  // 16 g + 4 j + c / 4.
+  static __device__ __forceinline__ typename Frag<T>::t col8(const T* base, int row, int col) {
+    const T* p = base + row * PITCH + col;
+    if constexpr (sizeof(T) == 4) {
       f32x8 v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = t[at(r0 + 8 * g + j, chunk) + (c & 3)];
+      for (int j = 0; j < 8; ++j) v[j] = p[tok(j) * PITCH];
       return v;
     } else {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef short s8 __attribute__((ext_vector_type(8)));
       typedef __attribute__((address_space(3))) s4* lds_s4;
-      const int row = r0 + 8 * g + ((lane & 15) >> 2), chunk = c0 / 8 + (lane & 3);
-      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + at(row, chunk) + 4 * half));
-      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + at(row + 4, chunk) + 4 * half));
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + PITCH));
       const s8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
       return __builtin_bit_cast(typename Frag<T>::t, v);
     }
   }
+  // P's tile (row c of a strip, columns col + 4 g .. + 3) into place
+  static __device__ __forceinline__ T* score_base(T* t, int c, int g) {
+    return sizeof(T) == 4 ? t + c * PITCH + 4 * g : t + c * PITCH + 8 * (g >> 1) + 2 * (g & 1);
+  }
+  static __device__ __forceinline__ void store_scores(T* base, int row, int col, const f32x4& p) {
+    T* d = base + row * PITCH + col;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(d) = make_float4(p[0], p[1], p[2], p[3]);
+    } else {
+      *reinterpret_cast<uint32_t*>(d) = pack2<T>(p[0], p[2]);
+      *reinterpret_cast<uint32_t*>(d + 4) = pack2<T>(p[1], p[3]);
+    }
+  }
+  static __device__ __forceinline__ const T* scores_base(const T* t, int c, int g) {
+    return sizeof(T) == 4 ? row44_base(t, c, g) : row8_base(t, c, g);
+  }
+  static __device__ __forceinline__ typename Frag<T>::t scores(const T* base, int row, int col) {
+    if constexpr (sizeof(T) == 4) return row44(base, row, col);
+    else return row8(base, row, col);
+  }
 };
+
+// A buffer descriptor over `bytes` bytes at `base`: loads past them return zeros.
+[[maybe_unused]] __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+[[maybe_unused]] constexpr uint32_t kOutside = 0xfffffff0u;  // an offset past every buffer
 
 // Rows of a tile on their way from memory to LDS, held in registers: the loads
 // of the next rows are issued before the products of the present ones.
@@ -108,34 +148,64 @@ template <typename T, int D, int ROWS, int THREADS>
 struct Stage {
   typedef Tile<T, D> L;
   static constexpr int N = ROWS * L::CPR / THREADS;
-  static_assert(ROWS * L::CPR % THREADS == 0, "whole chunks per thread");
+  static constexpr int RPT = THREADS / L::CPR;  // rows per turn of the threads
+  static_assert(ROWS * L::CPR % THREADS == 0 && THREADS % L::CPR == 0, "whole chunks per thread");
   uint4 v[N];
-  // rows [0, n) of `base`, `step` elements apart (negative: backwards), columns
-  // below d; zeros elsewhere
-  __device__ __forceinline__ void load(const T* base, int64_t step, int n, int d) {
+  // Row i of the tile is the n rows' i-th from `base`, or from their end
+  // (`back`); rows past n and columns past d are zeros.
+  __device__ __forceinline__ void load(const T* base, int64_t row_stride, int n, int d, bool back) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t step = (uint32_t)(row_stride * sizeof(T));
+    const __amdgpu_buffer_rsrc_t rs = buffer_of(base, (uint32_t)(n - 1) * step + (uint32_t)(d * sizeof(T)));
+    const int r = threadIdx.x / L::CPR, c = threadIdx.x % L::CPR;
+    uint32_t at = (uint32_t)(back ? n - 1 - r : r) * step + 16u * c;
+    const uint32_t turn = (back ? 0u - RPT : (uint32_t)RPT) * step;
+    const int lim = c * L::PER < d ? n - r : 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int q = i * THREADS + threadIdx.x, r = q / L::CPR, c = q % L::CPR;
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < n && c * L::PER < d) v[i] = ld16(base + r * step + c * L::PER);
+      const auto u = __builtin_amdgcn_raw_buffer_load_b128(rs, i * RPT < lim ? at : kOutside, 0, 0);
+      v[i] = make_uint4(u[0], u[1], u[2], u[3]);
+      at += turn;
     }
+#else
+    (void)base, (void)row_stride, (void)n, (void)d, (void)back;
+#endif
   }
   __device__ __forceinline__ void store(T* lds) const {
+    T* p = lds + threadIdx.x / L::CPR * L::PITCH + threadIdx.x % L::CPR * L::PER;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int q = i * THREADS + threadIdx.x;
-      st16(lds + L::at(q / L::CPR, q % L::CPR), v[i]);
-    }
+    for (int i = 0; i < N; ++i) st16(p + i * RPT * L::PITCH, v[i]);
   }
 };
 
+// Eight floats as operands of T: `rest` becomes what the operand leaves of
+// them (its high bits cut off, so that the next operand takes the following).
 template <typename T>
-__device__ __forceinline__ typename Frag<T>::t to_frag(const float* f) {
-  if constexpr (sizeof(T) == 4) {
-    return f32x8{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
-  } else {
-    return __builtin_bit_cast(typename Frag<T>::t, pack16<T>(f));
+__device__ __forceinline__ typename Frag<T>::t take(float (&rest)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    if constexpr (sizeof(T) == 2 && __is_same(T, bf16)) {
+      const uint32_t a = __builtin_bit_cast(uint32_t, rest[j]), b = __builtin_bit_cast(uint32_t, rest[j + 1]);
+      w[j / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      rest[j] -= __builtin_bit_cast(float, a & 0xffff0000u);
+      rest[j + 1] -= __builtin_bit_cast(float, b & 0xffff0000u);
+    } else {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(rest[j], rest[j + 1]);
+      w[j / 2] = __builtin_bit_cast(uint32_t, h);
+      rest[j] -= (float)h[0];
+      rest[j + 1] -= (float)h[1];
+    }
   }
+  return __builtin_bit_cast(typename Frag<T>::t, make_uint4(w[0], w[1], w[2], w[3]));
+}
+// Rounded to nearest: the last operand of a sum of them, or fp32 itself.
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::t to_frag(const float (&f)[8]) {
+  if constexpr (sizeof(T) == 4)
+    return f32x8{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+  else
+    return __builtin_bit_cast(typename Frag<T>::t, pack16<T>(f));
 }
 
 // ------------------------------------------------------------ the work items
@@ -167,6 +237,12 @@ __device__ __forceinline__ bool find_segment(const int32_t* __restrict__ cu, int
   if (s.index < 0 || s.index >= s.count) return false;
   s.row0 = a + (int64_t)s.index * seg;
   s.rows = (int)min<int64_t>(seg, b - s.row0);
+  // the same in every lane: addresses built on these stay scalar
+  s.seq = __builtin_amdgcn_readfirstlane(s.seq);
+  s.index = __builtin_amdgcn_readfirstlane(s.index);
+  s.count = __builtin_amdgcn_readfirstlane(s.count);
+  s.row0 = __builtin_amdgcn_readfirstlane((int)s.row0);  // below 2^30
+  s.rows = __builtin_amdgcn_readfirstlane(s.rows);
   return true;
 }
 
@@ -184,7 +260,7 @@ struct Role {
   int dx, dz;
   int reverse;
   int zero_tail;       // rows past the last sequence become zeros (gradients)
-  float pscale, oscale;
+  float p_mul, i_mul, z_mul;  // factors of P, of the state's share, of Z in the state's update
 };
 constexpr int kMaxRoles = 3;
 struct WalkArgs {
@@ -193,7 +269,7 @@ struct WalkArgs {
   const float* log_decay;
   int64_t total;
   int batch, kv_heads, seg, slots;
-  int terms;  // 16-bit terms the update's operand is split into (1 to 3)
+  int terms;  // 16-bit operands that a weighted row of Z is split into (2 or 3)
 };
 
 template <typename T, int DX> constexpr int chunk_rows() { return sizeof(T) == 4 && DX == 256 ? 32 : 64; }
@@ -201,12 +277,17 @@ template <typename T, int DX> constexpr int chunk_rows() { return sizeof(T) == 4
 template <typename T, int DX, int NW, bool OUT>
 constexpr size_t walk_lds() {
   constexpr int C = chunk_rows<T, DX>();
-  return sizeof(T) * (size_t)((OUT ? 2 : 1) * C * DX + C * 32 * NW + (OUT ? C * C : 0)) + 4 * (C + 4);
+  return sizeof(T) * (size_t)C * ((OUT ? 2 : 1) * Tile<T, DX>::PITCH + Tile<T, 32 * NW>::PITCH +
+                                  (OUT ? Tile<T, C>::PITCH : 0)) + 4 * (2 * C + 4);
 }
+// Waves per SIMD that the registers are held to: the state (DX / 2), out (C / 2)
+// and the staged rows fit 256 of them up to DX = 128; in fp32 the tiles fill
+// the LDS first.
+template <typename T> constexpr int walk_waves(int dx) { return dx <= (sizeof(T) == 4 ? 32 : 128) ? 2 : 1; }
 
 // NW waves; wave w owns columns [32 w, 32 w + 32) of z, out and the state.
 template <typename T, int DX, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW) void lin_walk_kernel(WalkArgs a) {
+__global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(WalkArgs a) {
   constexpr int C = chunk_rows<T, DX>();
   constexpr int DZ = 32 * NW, THREADS = 64 * NW;
   constexpr int ST = C / 16;  // strips of 16 rows
@@ -216,10 +297,10 @@ __global__ __launch_bounds__(64 * NW) void lin_walk_kernel(WalkArgs a) {
   typedef typename Frag<T>::t F;
   extern __shared__ __align__(16) char lds_raw[];
   T* ys = reinterpret_cast<T*>(lds_raw);
-  T* zs = ys + C * DX;
-  T* xs = zs + C * DZ;
-  T* ps = xs + (OUT ? C * DX : 0);
-  float* pow = reinterpret_cast<float*>(ps + (OUT ? C * C : 0));  // lam^0 .. lam^C
+  T* zs = ys + C * LX::PITCH;
+  T* xs = zs + C * LZ::PITCH;
+  T* ps = xs + (OUT ? C * LX::PITCH : 0);
+  float* pow = reinterpret_cast<float*>(ps + (OUT ? C * LP::PITCH : 0)) + C;  // [n]: z_mul lam^n; 0 for n < 0
 
   const Role& r = a.role[blockIdx.y];
   const int slices = (r.dz + DZ - 1) / DZ;
@@ -249,211 +330,260 @@ __global__ __launch_bounds__(64 * NW) void lin_walk_kernel(WalkArgs a) {
   }
   Segment sg;
   if (!find_segment(a.cu, a.batch, a.total, a.seg, slot, sg)) return;
-  const int first = r.reverse ? sg.count - 1 : 0, final = sg.count - 1 - first;
+  const bool back = r.reverse;
+  const int first = back ? sg.count - 1 : 0, final = sg.count - 1 - first;
   // a segment whose state nobody reads
   if (!OUT && (sg.index == final || sg.count == 1)) return;
+  const int rows = sg.rows, dx = r.dx;
+
+  const int y_group = r.y_group;
+  const T* x = static_cast<const T*>(r.x) + (OUT ? sg.row0 * r.x_row + head * r.x_head : 0);
+  const T* y = static_cast<const T*>(r.y) + sg.row0 * r.y_row + (int64_t)kvh * y_group * r.y_head;
+  const T* z = static_cast<const T*>(r.z) + sg.row0 * r.z_row + (int64_t)kvh * y_group * r.z_head + z0;
+  const int64_t x_row = r.x_row, y_row = r.y_row, z_row = r.z_row, y_head = r.y_head, z_head = r.z_head;
+  Stage<T, DX, C, THREADS> sx, sy;
+  Stage<T, DZ, C, THREADS> sz;
+  // chunk ci has n rows from row `low`: the walk's order from the segment's
+  // start, or from its end
+  auto chunk_rows_of = [&](int ci) { return min(C, rows - ci * C); };
+  auto chunk_low = [&](int ci, int n) { return (int64_t)(back ? rows - ci * C - n : ci * C); };
+  auto fetch = [&](int ci, int yg) {
+    const int n = chunk_rows_of(ci);
+    const int64_t low = chunk_low(ci, n);
+    sy.load(y + low * y_row + yg * y_head, y_row, n, dx, back);
+    sz.load(z + low * z_row + yg * z_head, z_row, n, zcols, back);
+    if constexpr (OUT) {
+      if (yg == 0) sx.load(x + low * x_row, x_row, n, dx, back);
+    }
+  };
+  const int chunks = (rows + C - 1) / C;
+  if (chunks) fetch(0, 0);
 
   const float g2 = a.log_decay[kvh] * 1.4426950408889634f;
   // lam^n; lam^0 is 1 also for a decay of -inf
-  auto power = [&](int n) { return n == 0 ? 1.f : exp2f(g2 * (float)n); };
-  for (int n = threadIdx.x; n <= C; n += THREADS) pow[n] = power(n);
-  const int e = r.reverse ? 0 : 1;
+  auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)n); };
+  for (int n = (int)threadIdx.x - C; n <= C; n += THREADS) pow[n] = n < 0 ? 0.f : power(n) * r.z_mul;
+  const int e = back ? 0 : 1;
 
-  // the state: element [2 s + t][u][i] is x-column 32 s + 8 g + 4 t + i,
-  // z-column 32 wave + 8 (c / 4) + 4 u + c % 4
+  // the state: element [m][u][i] is x-column 16 m + 4 g + i, z-column 32 wave + 16 u + c
   f32x4 st[DX / 16][2];
-  const int64_t state_size = (int64_t)r.dx * r.dz;
-  const int scol = 32 * wave + 8 * (c >> 2) + (c & 3);  // + 4 u
+  const int64_t state_size = (int64_t)dx * r.dz;
+  const int scol = 32 * wave + c;  // + 16 u
+  const bool whole = dx == DX && zcols == DZ;
   const float* in = nullptr;
   if constexpr (OUT) {
     if (sg.index != first) in = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
     else if (r.init) in = r.init + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
   }
+  if (in && whole) {
+    const float* p = in + 4 * g * r.s_x + (z0 + scol) * r.s_z;
 #pragma unroll
-  for (int m = 0; m < DX / 16; ++m)
+    for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int dx = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + i, dz = scol + 4 * u;
-        st[m][u][i] = in && dx < r.dx && dz < zcols ? in[dx * r.s_x + (z0 + dz) * r.s_z] : 0.f;
-      }
+        for (int i = 0; i < 4; ++i) st[m][u][i] = p[(16 * m + i) * r.s_x + 16 * u * r.s_z];
+  } else {
+#pragma unroll
+    for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int sx_ = 16 * m + 4 * g + i, sz_ = scol + 16 * u;
+          st[m][u][i] = in && sx_ < dx && sz_ < zcols ? in[sx_ * r.s_x + (z0 + sz_) * r.s_z] : 0.f;
+        }
+  }
 
   // weights of P's tiles, lane (c, g) element i: row t = c, column s = 4 g + i,
-  // tiles d strips below the diagonal
-  float wd[ST][4];
+  // tiles d strips below the diagonal; weights of the state's share, row c of a strip
+  float wd[OUT ? ST : 1][4], wi[OUT ? ST : 1];
+  if constexpr (OUT) {
 #pragma unroll
-  for (int d = 0; d < ST; ++d)
+    for (int d = 0; d < ST; ++d) {
+      wi[d] = power(16 * d + c + e) * r.i_mul;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int lag = 16 * d + c - (4 * g + i);
-      wd[d][i] = lag >= 0 ? power(lag) * r.pscale : 0.f;
-    }
-
-  const int64_t row_first = r.reverse ? sg.row0 + sg.rows - 1 : sg.row0;
-  const int64_t dir = r.reverse ? -1 : 1;
-  const T* x = static_cast<const T*>(r.x) + (OUT ? row_first * r.x_row + head * r.x_head : 0);
-  const T* y = static_cast<const T*>(r.y) + row_first * r.y_row + (int64_t)kvh * r.y_group * r.y_head;
-  const T* z = static_cast<const T*>(r.z) + row_first * r.z_row + (int64_t)kvh * r.y_group * r.z_head + z0;
-  Stage<T, DX, C, THREADS> sx, sy;
-  Stage<T, DZ, C, THREADS> sz;
-  const int chunks = (sg.rows + C - 1) / C, steps = chunks * r.y_group;
-  auto fetch = [&](int step) {
-    const int ci = step / r.y_group, yg = step % r.y_group;
-    const int64_t i0 = (int64_t)ci * C * dir;
-    const int n = min(C, sg.rows - ci * C);
-    sy.load(y + i0 * r.y_row + yg * r.y_head, dir * r.y_row, n, r.dx);
-    sz.load(z + i0 * r.z_row + yg * r.z_head, dir * r.z_row, n, zcols);
-    if constexpr (OUT) {
-      if (yg == 0) sx.load(x + i0 * r.x_row, dir * r.x_row, n, r.dx);
-    }
-  };
-  f32x4 o[2][ST];
-  if (steps) fetch(0);
-  for (int step = 0; step < steps; ++step) {
-    const int ci = step / r.y_group, yg = step % r.y_group;
-    const int n = min(C, sg.rows - ci * C);
-    sy.store(ys);
-    sz.store(zs);
-    if constexpr (OUT) {
-      if (yg == 0) sx.store(xs);
-    }
-    __syncthreads();
-    if (step + 1 < steps) fetch(step + 1);
-
-    if constexpr (OUT) {
-      // P, a strip of 16 rows per wave and turn, rounded to T for the product with Z
-#pragma unroll
-      for (int s0 = 0; s0 < ST; s0 += NW) {
-        const int strip = s0 + wave;
-        if (NW > ST && strip >= ST) break;
-        F xf[DX / 32];
-#pragma unroll
-        for (int k = 0; k < DX / 32; ++k) xf[k] = LX::row8(xs, 16 * strip + c, 32 * k + 8 * g);
-#pragma unroll
-        for (int tile = 0; tile < ST; ++tile) {
-          if (tile > (strip | 1)) continue;  // the products read pairs of tiles
-          f32x4 p = {0.f, 0.f, 0.f, 0.f};
-          if (tile <= strip) {
-#pragma unroll
-            for (int k = 0; k < DX / 32; ++k) mma(p, LX::row8(ys, 16 * tile + c, 32 * k + 8 * g), xf[k]);
-            const int d = strip - tile;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float w = 0.f;  // wd[d][i] without a run-time register index
-#pragma unroll
-              for (int j = 0; j < ST; ++j) w = d == j ? wd[j][i] : w;
-              p[i] *= w;
-            }
-          }
-          const int col = 16 * tile + 4 * g;
-          T* dst = ps + LP::at(16 * strip + c, col / LP::PER) + col % LP::PER;
-          if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4*>(dst) = make_float4(p[0], p[1], p[2], p[3]);
-          else
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int lag = 16 * d + c - (4 * g + i);
+        wd[d][i] = lag >= 0 ? power(lag) * r.p_mul : 0.f;
       }
-      // out^T = (X A)^T lam^{i+e}: the state's accumulators are its operand as they lie
-      if (yg == 0) {
+    }
+    // the products read P in pairs of tiles: those above the diagonal stay zero
+    for (int q = threadIdx.x; q < C * LP::PITCH / LP::PER; q += THREADS)
+      st16(ps + q * LP::PER, make_uint4(0u, 0u, 0u, 0u));
+  }
+  const float keep_whole = power(C);
+  const T *x8 = LX::row8_base(xs, c, g), *x44 = LX::row44_base(xs, c, g), *y8 = LX::row8_base(ys, c, g);
+  const T *yt = LX::col8_base(ys, c, g), *zt = LZ::col8_base(zs, c, g) + 32 * wave;
+  const T* p8 = LP::scores_base(ps, c, g);
+  T* pt = LP::score_base(ps, c, g);
+  const float* wz0 = pow - e - LX::TOK_G * g;
+
+  f32x4 o[2][OUT ? ST : 1];
+  for (int ci = 0; ci < chunks; ++ci) {
+    const int n = chunk_rows_of(ci);
+    for (int yg = 0; yg < y_group; ++yg) {
+      sy.store(ys);
+      sz.store(zs);
+      if constexpr (OUT) {
+        if (yg == 0) sx.store(xs);
+      }
+      __syncthreads();
+      if (yg + 1 < y_group) fetch(ci, yg + 1);
+      else if (ci + 1 < chunks) fetch(ci + 1, 0);
+
+      if constexpr (OUT) {
+        // P, strips of 16 rows in turn over the waves, rounded to T
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int s0 = 0; s0 < ST; s0 += NW) {
+          const int strip = s0 + wave;
+          if (NW > ST && strip >= ST) break;
+          F xf[DX / 32];
 #pragma unroll
-          for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int k = 0; k < DX / 32; ++k) xf[k] = LX::row8(x8, 16 * strip, 32 * k);
 #pragma unroll
-        for (int k = 0; k < DX / 32; ++k) {
-          F sf[2];
+          for (int d = 0; d < ST; ++d) {
+            if (d > strip) break;
+            const int tile = strip - d;
+            f32x4 p = {0.f, 0.f, 0.f, 0.f};
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float f[8];
+            for (int k = 0; k < DX / 32; ++k) mma(p, LX::row8(y8, 16 * tile, 32 * k), xf[k]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[i] = st[2 * k][u][i];
-              f[4 + i] = st[2 * k + 1][u][i];
+            for (int i = 0; i < 4; ++i) p[i] *= wd[d][i];
+            LP::store_scores(pt, 16 * strip, 16 * tile, p);
+          }
+        }
+        // out^T = (X A)^T lam^{i+e}: the state's accumulators are its operand as
+        // they lie, in two 16-bit operands
+        if (yg == 0) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < DX / 32; ++k) {
+            // reads hoisted over several k would not fit the registers
+            __builtin_amdgcn_sched_barrier(0);
+            F xf[ST];
+#pragma unroll
+            for (int s = 0; s < ST; ++s) xf[s] = LX::row44(x44, 16 * s, 32 * k);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float f[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                f[i] = st[2 * k][u][i];
+                f[4 + i] = st[2 * k + 1][u][i];
+              }
+              if constexpr (sizeof(T) == 2) {
+                const F hi = take<T>(f);
+#pragma unroll
+                for (int s = 0; s < ST; ++s) mma(o[u][s], hi, xf[s]);
+              }
+              const F lo = to_frag<T>(f);
+#pragma unroll
+              for (int s = 0; s < ST; ++s) mma(o[u][s], lo, xf[s]);
             }
-            sf[u] = to_frag<T>(f);
           }
 #pragma unroll
           for (int s = 0; s < ST; ++s) {
-            const F xf = LX::row8(xs, 16 * s + c, 32 * k + 8 * g);
-            mma(o[0][s], sf[0], xf);
-            mma(o[1][s], sf[1], xf);
+            o[0][s] *= wi[s];
+            o[1][s] *= wi[s];
           }
         }
+        __syncthreads();
+      }
+      if (yg == 0) {
+        const float w = n == C ? keep_whole : power(n);
 #pragma unroll
-        for (int s = 0; s < ST; ++s) {
-          const float w = pow[16 * s + c + e];
-          o[0][s] *= w;
-          o[1][s] *= w;
+        for (int m = 0; m < DX / 16; ++m) {
+          st[m][0] *= w;
+          st[m][1] *= w;
+        }
+      }
+      const float* wz = wz0 + n;
+#pragma unroll
+      for (int kk = 0; kk < C / 32; ++kk) {
+        __builtin_amdgcn_sched_barrier(0);
+        const F zf[2] = {LZ::col8(zt, 32 * kk, 0), LZ::col8(zt, 32 * kk, 16)};
+        if constexpr (OUT) {
+#pragma unroll
+          for (int s = 2 * kk; s < ST; ++s) {
+            const F pf = LP::scores(p8, 16 * s, 32 * kk);
+            mma(o[0][s], zf[0], pf);
+            mma(o[1][s], zf[1], pf);
+          }
+        }
+        // Z weighted by lam^{n - e - i}, in two or three 16-bit operands
+        float rest[2][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float w = wz[-(32 * kk + LX::tok(j))];
+          rest[0][j] = (float)zf[0][j] * w;
+          rest[1][j] = (float)zf[1][j] * w;
+        }
+        if constexpr (sizeof(T) == 2) {
+          F hi[2] = {take<T>(rest[0]), take<T>(rest[1])};
+          if (a.terms > 2) {
+#pragma unroll
+            for (int m = 0; m < DX / 16; ++m) {
+              const F yf = LX::col8(yt, 32 * kk, 16 * m);
+              mma(st[m][0], yf, hi[0]);
+              mma(st[m][1], yf, hi[1]);
+            }
+            hi[0] = take<T>(rest[0]);
+            hi[1] = take<T>(rest[1]);
+          }
+          const F lo[2] = {to_frag<T>(rest[0]), to_frag<T>(rest[1])};
+#pragma unroll
+          for (int m = 0; m < DX / 16; ++m) {
+            if (m % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+            const F yf = LX::col8(yt, 32 * kk, 16 * m);
+            mma(st[m][0], yf, hi[0]);
+            mma(st[m][1], yf, hi[1]);
+            mma(st[m][0], yf, lo[0]);
+            mma(st[m][1], yf, lo[1]);
+          }
+        } else {
+          const F zw[2] = {to_frag<T>(rest[0]), to_frag<T>(rest[1])};
+#pragma unroll
+          for (int m = 0; m < DX / 16; ++m) {
+            if (m % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+            const F yf = LX::col8(yt, 32 * kk, 16 * m);
+            mma(st[m][0], yf, zw[0]);
+            mma(st[m][1], yf, zw[1]);
+          }
         }
       }
       __syncthreads();
     }
-    if (yg == 0) {
-      const float w = pow[n];
-#pragma unroll
-      for (int m = 0; m < DX / 16; ++m) {
-        st[m][0] *= w;
-        st[m][1] *= w;
-      }
-    }
-#pragma unroll
-    for (int kk = 0; kk < C / 32; ++kk) {
-      const F zf[2] = {LZ::col8(zs, 32 * kk, 32 * wave, 0), LZ::col8(zs, 32 * kk, 32 * wave, 1)};
-      if constexpr (OUT) {
-#pragma unroll
-        for (int s = 2 * kk; s < ST; ++s) {
-          const F pf = LP::row8(ps, 16 * s + c, 32 * kk + 8 * g);
-          mma(o[0][s], zf[0], pf);
-          mma(o[1][s], zf[1], pf);
-        }
-      }
-      // Z weighted by lam^{n - e - i}, rounded to T (in `terms` terms, each the
-      // rounding of what the ones before leave)
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = pow[max(0, n - e - (32 * kk + 8 * g + j))] * r.pscale;
-      float rest[2][8];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rest[u][j] = (float)zf[u][j] * w[j];
-      for (int t = 0; t < (sizeof(T) == 4 ? 1 : a.terms); ++t) {
-        F zw[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          zw[u] = to_frag<T>(rest[u]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) rest[u][j] -= (float)zw[u][j];
-        }
-#pragma unroll
-        for (int m = 0; m < DX / 16; ++m) {
-          const F yf = LX::col8(ys, 32 * kk, 32 * (m >> 1), m & 1);
-          mma(st[m][0], yf, zw[0]);
-          mma(st[m][1], yf, zw[1]);
-        }
-      }
-    }
     if constexpr (OUT) {
-      if (yg == r.y_group - 1 && 32 * wave + 8 * g < zcols) {
+      const int64_t low = chunk_low(ci, n);
+      T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + head * r.o_head + z0;
 #pragma unroll
-        for (int s = 0; s < ST; ++s) {
-          const int i = 16 * s + c;
-          if (i >= n) continue;
-          T* out = static_cast<T*>(r.out) + (row_first + dir * ((int64_t)ci * C + i)) * r.o_row +
-                   head * r.o_head + z0 + 32 * wave + 8 * g;
-          float f[8];
+      for (int s = 0; s < ST; ++s) {
+        const int i = 16 * s + c;
+        T* dst = out + (int64_t)(back ? n - 1 - i : i) * r.o_row;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f[k] = o[0][s][k] * r.oscale;
-            f[4 + k] = o[1][s][k] * r.oscale;
+          for (int u = 0; u < 2; ++u) {
+            const int col = 32 * wave + 16 * u + 4 * g;
+            if (i < n && col < zcols)
+              *reinterpret_cast<float4*>(dst + col) = make_float4(o[u][s][0], o[u][s][1], o[u][s][2], o[u][s][3]);
           }
-          st16(out, pack16<T>(f));
-          if constexpr (sizeof(T) == 4) st16(out + 4, pack16<T>(f + 4));
+        } else {
+          // lanes of group g hold 4 columns of either half; exchanged between
+          // neighbouring groups they hold 8 in a row
+          uint32_t a0 = pack2<T>(o[0][s][0], o[0][s][1]), a1 = pack2<T>(o[0][s][2], o[0][s][3]);
+          uint32_t b0 = pack2<T>(o[1][s][0], o[1][s][1]), b1 = pack2<T>(o[1][s][2], o[1][s][3]);
+          const auto e0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
+          const auto e1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
+          const int col = 32 * wave + 16 * (g & 1) + 8 * (g >> 1);
+          if (i < n && col < zcols) st16(dst + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
         }
       }
     }
-    __syncthreads();
   }
 
   float* to = nullptr;
@@ -464,14 +594,18 @@ __global__ __launch_bounds__(64 * NW) void lin_walk_kernel(WalkArgs a) {
       to = r.last + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
   }
   if (!to) return;
+  // the places of the state's load, computed again: kept over the walk they
+  // would take its registers
+  int g_ = g, c_ = c;
+  asm volatile("" : "+v"(g_), "+v"(c_));
 #pragma unroll
   for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int dx = 32 * (m >> 1) + 8 * g + 4 * (m & 1) + i, dz = scol + 4 * u;
-        if (dx < r.dx && dz < zcols) to[dx * r.s_x + (z0 + dz) * r.s_z] = st[m][u][i];
+        const int sx_ = 16 * m + 4 * g_ + i, sz_ = 32 * wave + c_ + 16 * u;
+        if (whole || (sx_ < dx && sz_ < zcols)) to[sx_ * r.s_x + (z0 + sz_) * r.s_z] = st[m][u][i];
       }
 }
 
@@ -713,9 +847,12 @@ int launch_walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream
 }
 template <typename T, bool OUT, int DX>
 int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
+  // waves enough for z's columns, and for the rows staged in their registers
   const int dz = a.role[0].dz;
-  if (dz <= 32) return launch_walk<T, DX, 1, OUT>(fn, a, roles, stream);
-  if (dz <= 64) return launch_walk<T, DX, 2, OUT>(fn, a, roles, stream);
+  if constexpr (DX <= 32)
+    if (dz <= 32) return launch_walk<T, DX, 1, OUT>(fn, a, roles, stream);
+  if constexpr (DX <= 64)
+    if (dz <= 64) return launch_walk<T, DX, 2, OUT>(fn, a, roles, stream);
   return launch_walk<T, DX, 4, OUT>(fn, a, roles, stream);
 }
 // One launch for `roles` walks of equal dims.
@@ -752,13 +889,10 @@ WalkArgs common_args(const Shape& s, const int32_t* cu, const float* log_decay, 
   return a;
 }
 
-// 16-bit terms of the weighted operand in the states' updates: one where a
-// state only feeds outputs of the same 16 bits, enough for fp32 where it is
+// 16-bit operands of a weighted row in the states' updates: 16 (bf16) or 22
+// (fp16) bits where a state only feeds 16-bit outputs, fp32's 24 where it is
 // an output itself.
-int update_terms(int dtype, bool state_out) {
-  if (!state_out) return 1;
-  return dtype == SCREE_DTYPE_BF16 ? 3 : 2;
-}
+int update_terms(int dtype, bool state_out) { return state_out && dtype == SCREE_DTYPE_BF16 ? 3 : 2; }
 
 template <typename T>
 int run_fwd(const char* fn, const Shape& s, const void* q, const void* k, const void* v, void* o,
@@ -768,7 +902,7 @@ int run_fwd(const char* fn, const Shape& s, const void* q, const void* k, const 
   const int group = s.heads / s.kv_heads;
   a.role[0] = {q, k, v, o, st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7],
                init, last, static_cast<float*>(workspace), s.dv, 1,
-               s.heads, group, 1, s.dk, s.dv, 0, 0, 1.f, scale};
+               s.heads, group, 1, s.dk, s.dv, 0, 0, scale, scale, 1.f};
   if (s.total > a.seg)
     if (int rc = segment_states<T>(fn, a, 1, stream)) return rc;
   return walk<T, true>(fn, a, 1, stream);
@@ -787,17 +921,17 @@ int run_bwd(const char* fn, const Shape& s, const void* dout, const void* q, con
   if (s.total > a.seg) {
     // S forward from (k, v), R backward from (q, dout), both dk x dv
     a.role[0] = {nullptr, k, v, nullptr, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0,
-                 init, nullptr, seg_s, s.dv, 1, s.heads, group, 1, s.dk, s.dv, 0, 0, 1.f, 1.f};
+                 init, nullptr, seg_s, s.dv, 1, s.heads, group, 1, s.dk, s.dv, 0, 0, 1.f, 1.f, 1.f};
     a.role[1] = {nullptr, q, dout, nullptr, 0, 0, sq[0], sq[1], sdo[0], sdo[1], 0, 0,
-                 dlast, nullptr, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 0, scale, 1.f};
+                 dlast, nullptr, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 0, 1.f, 1.f, scale};
     if (int rc = segment_states<T>(fn, a, 2, stream)) return rc;
   }
   const Role rdq = {dout, v, k, dq, sdo[0], sdo[1], sv[0], sv[1], sk[0], sk[1], sdq[0], sdq[1],
-                    init, nullptr, seg_s, 1, s.dv, s.heads, group, 1, s.dv, s.dk, 0, 1, 1.f, scale};
+                    init, nullptr, seg_s, 1, s.dv, s.heads, group, 1, s.dv, s.dk, 0, 1, scale, scale, 1.f};
   const Role rdk = {v, dout, q, dk, sv[0], sv[1], sdo[0], sdo[1], sq[0], sq[1], sdk[0], sdk[1],
-                    dlast, nullptr, seg_r, 1, s.dv, s.kv_heads, 1, group, s.dv, s.dk, 1, 1, scale, 1.f};
+                    dlast, nullptr, seg_r, 1, s.dv, s.kv_heads, 1, group, s.dv, s.dk, 1, 1, scale, 1.f, scale};
   const Role rdv = {k, q, dout, dv, sk[0], sk[1], sq[0], sq[1], sdo[0], sdo[1], sdv[0], sdv[1],
-                    dlast, dinit, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 1, scale, 1.f};
+                    dlast, dinit, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 1, scale, 1.f, scale};
   a.role[0] = rdk;
   a.role[1] = rdq;
   a.role[2] = rdv;
