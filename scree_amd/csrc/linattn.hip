@@ -277,20 +277,27 @@ template <typename T, int DX> constexpr int chunk_rows() { return sizeof(T) == 4
 template <typename T, int DX, int NW, bool OUT>
 constexpr size_t walk_lds() {
   constexpr int C = chunk_rows<T, DX>();
-  return sizeof(T) * (size_t)C * ((OUT ? 2 : 1) * Tile<T, DX>::PITCH + Tile<T, 32 * NW>::PITCH +
-                                  (OUT ? Tile<T, C>::PITCH : 0)) + 4 * (2 * C + 4);
+  return sizeof(T) * (size_t)C * ((OUT ? 2 : 1) * Tile<T, DX>::PITCH + Tile<T, 16 * NW>::PITCH +
+                                  (OUT ? Tile<T, C>::PITCH : 0)) +
+         sizeof(float) * (OUT ? 3 : 1) * 2 * (C + 4);
 }
-// Waves per SIMD that the registers are held to: the state (DX / 2), out (C / 2)
-// and the staged rows fit 256 of them up to DX = 128; in fp32 the tiles fill
-// the LDS first.
-template <typename T> constexpr int walk_waves(int dx) { return dx <= (sizeof(T) == 4 ? 32 : 128) ? 2 : 1; }
-
-// NW waves; wave w owns columns [32 w, 32 w + 32) of z, out and the state.
+// Waves per SIMD that the registers are held to: as many as the LDS leaves room
+// for, four at most (128 registers).
 template <typename T, int DX, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(WalkArgs a) {
+constexpr int walk_waves() {
+  const int w = (int)(160 * 1024 / walk_lds<T, DX, NW, OUT>()) * NW / 4;
+  return w < 1 ? 1 : w > 4 ? 4 : w;
+}
+
+// NW waves; wave w owns columns [16 w, 16 w + 16) of z, out and the state.
+// Two waves to a SIMD with 32 columns each (half the LDS reads, twice the
+// registers) ran 1.5x longer: what bounds the walk is waiting.
+template <typename T, int DX, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_walk_kernel(WalkArgs a) {
   constexpr int C = chunk_rows<T, DX>();
-  constexpr int DZ = 32 * NW, THREADS = 64 * NW;
-  constexpr int ST = C / 16;  // strips of 16 rows
+  constexpr int DZ = 16 * NW, THREADS = 64 * NW;
+  constexpr int ST = C / 16;                   // strips of 16 rows
+  constexpr int WPS = NW > ST ? NW / ST : 1;   // waves that share a strip of P
   typedef Tile<T, DX> LX;
   typedef Tile<T, DZ> LZ;
   typedef Tile<T, C> LP;
@@ -300,7 +307,10 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(Wa
   T* zs = ys + C * LX::PITCH;
   T* xs = zs + C * LZ::PITCH;
   T* ps = xs + (OUT ? C * LX::PITCH : 0);
-  float* pow = reinterpret_cast<float*>(ps + (OUT ? C * LP::PITCH : 0)) + C;  // [n]: z_mul lam^n; 0 for n < 0
+  // lam^n, -C <= n <= C, 0 for n < 0: times z_mul, p_mul and i_mul
+  float* pow = reinterpret_cast<float*>(ps + (OUT ? C * LP::PITCH : 0)) + C;
+  float* pow_p = pow + (OUT ? 2 * (C + 4) : 0);
+  float* pow_i = pow_p + (OUT ? 2 * (C + 4) : 0);
 
   const Role& r = a.role[blockIdx.y];
   const int slices = (r.dz + DZ - 1) / DZ;
@@ -362,64 +372,57 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(Wa
   const float g2 = a.log_decay[kvh] * 1.4426950408889634f;
   // lam^n; lam^0 is 1 also for a decay of -inf
   auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)n); };
-  for (int n = (int)threadIdx.x - C; n <= C; n += THREADS) pow[n] = n < 0 ? 0.f : power(n) * r.z_mul;
+  for (int n = (int)threadIdx.x - C; n <= C; n += THREADS) {
+    const float w = n < 0 ? 0.f : power(n);
+    pow[n] = w * r.z_mul;
+    if constexpr (OUT) {
+      pow_p[n] = w * r.p_mul;
+      pow_i[n] = w * r.i_mul;
+    }
+  }
   const int e = back ? 0 : 1;
 
-  // the state: element [m][u][i] is x-column 16 m + 4 g + i, z-column 32 wave + 16 u + c
-  f32x4 st[DX / 16][2];
+  // the state: element [m][i] is x-column 16 m + 4 g + i, z-column 16 wave + c
+  f32x4 st[DX / 16];
   const int64_t state_size = (int64_t)dx * r.dz;
-  const int scol = 32 * wave + c;  // + 16 u
   const bool whole = dx == DX && zcols == DZ;
   const float* in = nullptr;
   if constexpr (OUT) {
     if (sg.index != first) in = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
     else if (r.init) in = r.init + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
   }
-  if (in && whole) {
-    const float* p = in + 4 * g * r.s_x + (z0 + scol) * r.s_z;
+  if (in) {
+    const float* p = in + 4 * g * r.s_x + (z0 + 16 * wave + c) * r.s_z;
+    const bool col = 16 * wave + c < zcols;
 #pragma unroll
     for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st[m][u][i] = p[(16 * m + i) * r.s_x + 16 * u * r.s_z];
+      for (int i = 0; i < 4; ++i)
+        st[m][i] = whole || (col && 16 * m + 4 * g + i < dx) ? p[(16 * m + i) * r.s_x] : 0.f;
   } else {
 #pragma unroll
-    for (int m = 0; m < DX / 16; ++m)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int sx_ = 16 * m + 4 * g + i, sz_ = scol + 16 * u;
-          st[m][u][i] = in && sx_ < dx && sz_ < zcols ? in[sx_ * r.s_x + (z0 + sz_) * r.s_z] : 0.f;
-        }
+    for (int m = 0; m < DX / 16; ++m) st[m] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // weights of P's tiles, lane (c, g) element i: row t = c, column s = 4 g + i,
-  // tiles d strips below the diagonal; weights of the state's share, row c of a strip
-  float wd[OUT ? ST : 1][4], wi[OUT ? ST : 1];
   if constexpr (OUT) {
-#pragma unroll
-    for (int d = 0; d < ST; ++d) {
-      wi[d] = power(16 * d + c + e) * r.i_mul;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int lag = 16 * d + c - (4 * g + i);
-        wd[d][i] = lag >= 0 ? power(lag) * r.p_mul : 0.f;
-      }
-    }
     // the products read P in pairs of tiles: those above the diagonal stay zero
     for (int q = threadIdx.x; q < C * LP::PITCH / LP::PER; q += THREADS)
       st16(ps + q * LP::PER, make_uint4(0u, 0u, 0u, 0u));
   }
   const float keep_whole = power(C);
   const T *x8 = LX::row8_base(xs, c, g), *x44 = LX::row44_base(xs, c, g), *y8 = LX::row8_base(ys, c, g);
-  const T *yt = LX::col8_base(ys, c, g), *zt = LZ::col8_base(zs, c, g) + 32 * wave;
+  const T *yt = LX::col8_base(ys, c, g), *zt = LZ::col8_base(zs, c, g) + 16 * wave;
   const T* p8 = LP::scores_base(ps, c, g);
   T* pt = LP::score_base(ps, c, g);
+  // weights of P's tiles d strips below the diagonal, lane (c, g) element i: row
+  // t = c, column s = 4 g + i, lam^{16 d + c - 4 g - i}; of the state's share,
+  // row c of strip s, lam^{16 s + c + e}
+  const float *wp = pow_p + c - 4 * g, *wi = pow_i + c + e;
   const float* wz0 = pow - e - LX::TOK_G * g;
+  // operands of a weighted row: an output state gets as many as fp32 has bits for
+  const bool three = sizeof(T) == 2 && a.terms > 2 && (!OUT || sg.index == final);
 
-  f32x4 o[2][OUT ? ST : 1];
+  f32x4 o[OUT ? ST : 1];
   for (int ci = 0; ci < chunks; ++ci) {
     const int n = chunk_rows_of(ci);
     for (int yg = 0; yg < y_group; ++yg) {
@@ -433,24 +436,22 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(Wa
       else if (ci + 1 < chunks) fetch(ci + 1, 0);
 
       if constexpr (OUT) {
-        // P, strips of 16 rows in turn over the waves, rounded to T
+        // P, a strip of 16 rows to WPS waves (every WPS-th tile each), rounded to T
 #pragma unroll
         for (int s0 = 0; s0 < ST; s0 += NW) {
-          const int strip = s0 + wave;
-          if (NW > ST && strip >= ST) break;
+          const int strip = s0 + wave / WPS;
           F xf[DX / 32];
 #pragma unroll
           for (int k = 0; k < DX / 32; ++k) xf[k] = LX::row8(x8, 16 * strip, 32 * k);
 #pragma unroll
           for (int d = 0; d < ST; ++d) {
-            if (d > strip) break;
+            if (d > strip || (WPS > 1 && d % WPS != wave % WPS)) continue;
             const int tile = strip - d;
             f32x4 p = {0.f, 0.f, 0.f, 0.f};
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < DX / 32; ++k) mma(p, LX::row8(y8, 16 * tile, 32 * k), xf[k]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] *= wd[d][i];
+            for (int i = 0; i < 4; ++i) p[i] *= wp[16 * d - i];
             LP::store_scores(pt, 16 * strip, 16 * tile, p);
           }
         }
@@ -458,9 +459,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(Wa
         // they lie, in two 16-bit operands
         if (yg == 0) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int s = 0; s < ST; ++s) o[s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < DX / 32; ++k) {
             // reads hoisted over several k would not fit the registers
@@ -468,119 +467,91 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(Wa
             F xf[ST];
 #pragma unroll
             for (int s = 0; s < ST; ++s) xf[s] = LX::row44(x44, 16 * s, 32 * k);
+            float f[8];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float f[8];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                f[i] = st[2 * k][u][i];
-                f[4 + i] = st[2 * k + 1][u][i];
-              }
-              if constexpr (sizeof(T) == 2) {
-                const F hi = take<T>(f);
-#pragma unroll
-                for (int s = 0; s < ST; ++s) mma(o[u][s], hi, xf[s]);
-              }
-              const F lo = to_frag<T>(f);
-#pragma unroll
-              for (int s = 0; s < ST; ++s) mma(o[u][s], lo, xf[s]);
+            for (int i = 0; i < 4; ++i) {
+              f[i] = st[2 * k][i];
+              f[4 + i] = st[2 * k + 1][i];
             }
+            if constexpr (sizeof(T) == 2) {
+              const F hi = take<T>(f);
+#pragma unroll
+              for (int s = 0; s < ST; ++s) mma(o[s], hi, xf[s]);
+            }
+            const F lo = to_frag<T>(f);
+#pragma unroll
+            for (int s = 0; s < ST; ++s) mma(o[s], lo, xf[s]);
           }
 #pragma unroll
-          for (int s = 0; s < ST; ++s) {
-            o[0][s] *= wi[s];
-            o[1][s] *= wi[s];
-          }
+          for (int s = 0; s < ST; ++s) o[s] *= wi[16 * s];
         }
         __syncthreads();
       }
       if (yg == 0) {
         const float w = n == C ? keep_whole : power(n);
 #pragma unroll
-        for (int m = 0; m < DX / 16; ++m) {
-          st[m][0] *= w;
-          st[m][1] *= w;
-        }
+        for (int m = 0; m < DX / 16; ++m) st[m] *= w;
       }
       const float* wz = wz0 + n;
 #pragma unroll
       for (int kk = 0; kk < C / 32; ++kk) {
         __builtin_amdgcn_sched_barrier(0);
-        const F zf[2] = {LZ::col8(zt, 32 * kk, 0), LZ::col8(zt, 32 * kk, 16)};
+        const F zf = LZ::col8(zt, 32 * kk, 0);
         if constexpr (OUT) {
 #pragma unroll
-          for (int s = 2 * kk; s < ST; ++s) {
-            const F pf = LP::scores(p8, 16 * s, 32 * kk);
-            mma(o[0][s], zf[0], pf);
-            mma(o[1][s], zf[1], pf);
-          }
+          for (int s = 2 * kk; s < ST; ++s) mma(o[s], zf, LP::scores(p8, 16 * s, 32 * kk));
         }
         // Z weighted by lam^{n - e - i}, in two or three 16-bit operands
-        float rest[2][8];
+        float rest[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = wz[-(32 * kk + LX::tok(j))];
-          rest[0][j] = (float)zf[0][j] * w;
-          rest[1][j] = (float)zf[1][j] * w;
-        }
+        for (int j = 0; j < 8; ++j) rest[j] = (float)zf[j] * wz[-(32 * kk + LX::tok(j))];
         if constexpr (sizeof(T) == 2) {
-          F hi[2] = {take<T>(rest[0]), take<T>(rest[1])};
-          if (a.terms > 2) {
+          F hi = take<T>(rest);
+          if (three) {
 #pragma unroll
-            for (int m = 0; m < DX / 16; ++m) {
-              const F yf = LX::col8(yt, 32 * kk, 16 * m);
-              mma(st[m][0], yf, hi[0]);
-              mma(st[m][1], yf, hi[1]);
-            }
-            hi[0] = take<T>(rest[0]);
-            hi[1] = take<T>(rest[1]);
+            for (int m = 0; m < DX / 16; ++m) mma(st[m], LX::col8(yt, 32 * kk, 16 * m), hi);
+            hi = take<T>(rest);
           }
-          const F lo[2] = {to_frag<T>(rest[0]), to_frag<T>(rest[1])};
+          const F lo = to_frag<T>(rest);
 #pragma unroll
           for (int m = 0; m < DX / 16; ++m) {
             if (m % 4 == 0) __builtin_amdgcn_sched_barrier(0);
             const F yf = LX::col8(yt, 32 * kk, 16 * m);
-            mma(st[m][0], yf, hi[0]);
-            mma(st[m][1], yf, hi[1]);
-            mma(st[m][0], yf, lo[0]);
-            mma(st[m][1], yf, lo[1]);
+            mma(st[m], yf, hi);
+            mma(st[m], yf, lo);
           }
         } else {
-          const F zw[2] = {to_frag<T>(rest[0]), to_frag<T>(rest[1])};
+          const F zw = to_frag<T>(rest);
 #pragma unroll
-          for (int m = 0; m < DX / 16; ++m) {
-            if (m % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-            const F yf = LX::col8(yt, 32 * kk, 16 * m);
-            mma(st[m][0], yf, zw[0]);
-            mma(st[m][1], yf, zw[1]);
-          }
+          for (int m = 0; m < DX / 16; ++m) mma(st[m], LX::col8(yt, 32 * kk, 16 * m), zw);
         }
       }
       __syncthreads();
     }
     if constexpr (OUT) {
       const int64_t low = chunk_low(ci, n);
-      T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + head * r.o_head + z0;
+      T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + head * r.o_head + z0 + 16 * wave;
+      // row i of the chunk lies at i, or at n - 1 - i
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int s = 0; s < ST; ++s) {
-        const int i = 16 * s + c;
-        T* dst = out + (int64_t)(back ? n - 1 - i : i) * r.o_row;
-        if constexpr (sizeof(T) == 4) {
+        for (int s = 0; s < ST; ++s) {
+          const int i = 16 * s + c;
+          if (i < n && 16 * wave + 4 * g < zcols)
+            *reinterpret_cast<float4*>(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + 4 * g) =
+                make_float4(o[s][0], o[s][1], o[s][2], o[s][3]);
+        }
+      } else {
+        // a lane holds 4 columns of a row in every strip; exchanged between two
+        // strips and neighbouring groups, 8 columns of a row in one of the two
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int col = 32 * wave + 16 * u + 4 * g;
-            if (i < n && col < zcols)
-              *reinterpret_cast<float4*>(dst + col) = make_float4(o[u][s][0], o[u][s][1], o[u][s][2], o[u][s][3]);
-          }
-        } else {
-          // lanes of group g hold 4 columns of either half; exchanged between
-          // neighbouring groups they hold 8 in a row
-          uint32_t a0 = pack2<T>(o[0][s][0], o[0][s][1]), a1 = pack2<T>(o[0][s][2], o[0][s][3]);
-          uint32_t b0 = pack2<T>(o[1][s][0], o[1][s][1]), b1 = pack2<T>(o[1][s][2], o[1][s][3]);
-          const auto e0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
-          const auto e1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
-          const int col = 32 * wave + 16 * (g & 1) + 8 * (g >> 1);
-          if (i < n && col < zcols) st16(dst + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
+        for (int s = 0; s < ST; s += 2) {
+          const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[s][0], o[s][1]), pack2<T>(o[s + 1][0], o[s + 1][1]),
+                                                           false, false);
+          const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[s][2], o[s][3]), pack2<T>(o[s + 1][2], o[s + 1][3]),
+                                                           false, false);
+          const int i = 16 * (s + (g & 1)) + c, col = 8 * (g >> 1);
+          if (i < n && 16 * wave + col < zcols)
+            st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
         }
       }
     }
@@ -598,15 +569,13 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(DX)) void lin_walk_kernel(Wa
   // would take its registers
   int g_ = g, c_ = c;
   asm volatile("" : "+v"(g_), "+v"(c_));
+  to += 4 * g_ * r.s_x + (z0 + 16 * wave + c_) * r.s_z;
+  const bool col = 16 * wave + c_ < zcols;
 #pragma unroll
   for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int sx_ = 16 * m + 4 * g_ + i, sz_ = 32 * wave + c_ + 16 * u;
-        if (whole || (sx_ < dx && sz_ < zcols)) to[sx_ * r.s_x + (z0 + sz_) * r.s_z] = st[m][u][i];
-      }
+    for (int i = 0; i < 4; ++i)
+      if (whole || (col && 16 * m + 4 * g_ + i < dx)) to[(16 * m + i) * r.s_x] = st[m][i];
 }
 
 // The segments' own states become the states that come into them: along each
@@ -829,7 +798,7 @@ int launch_walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream
   int64_t items = 0;
   for (int i = 0; i < roles; ++i) {
     const Role& r = a.role[i];
-    const int64_t n = (int64_t)a.slots * (OUT ? r.heads : a.kv_heads) * ((r.dz + 32 * NW - 1) / (32 * NW));
+    const int64_t n = (int64_t)a.slots * (OUT ? r.heads : a.kv_heads) * ((r.dz + 16 * NW - 1) / (16 * NW));
     if (n > items) items = n;
   }
   if (items * 64 * NW > 0xffffffffll)
@@ -849,11 +818,11 @@ template <typename T, bool OUT, int DX>
 int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
   // waves enough for z's columns, and for the rows staged in their registers
   const int dz = a.role[0].dz;
-  if constexpr (DX <= 32)
-    if (dz <= 32) return launch_walk<T, DX, 1, OUT>(fn, a, roles, stream);
   if constexpr (DX <= 64)
-    if (dz <= 64) return launch_walk<T, DX, 2, OUT>(fn, a, roles, stream);
-  return launch_walk<T, DX, 4, OUT>(fn, a, roles, stream);
+    if (dz <= 32) return launch_walk<T, DX, 2, OUT>(fn, a, roles, stream);
+  if constexpr (DX <= 128)
+    if (DX <= 32 || dz <= 64) return launch_walk<T, DX, 4, OUT>(fn, a, roles, stream);
+  if constexpr (DX > 32) return launch_walk<T, DX, 8, OUT>(fn, a, roles, stream);
 }
 // One launch for `roles` walks of equal dims.
 template <typename T, bool OUT>
