@@ -65,9 +65,21 @@ struct Tile {
   }
   static constexpr int TOK_G = sizeof(T) == 4 ? 4 : 8;  // the group's part: TOK_G g
 
+  // X is read twice: in the order in which two accumulators hold 32 rows
+  // (columns 4 g .. + 3 and 16 + 4 g .. + 3 of 32) and in order.  In 16 bits it
+  // lies so that the first is one read: 4 columns u = 0 .. 7 of 32 at place
+  // 2 (u % 4) + u / 4.  (Two 8-byte reads in place of the one met in the banks:
+  // 16 LDS cycles against 5.)
+  static constexpr bool kPairs = sizeof(T) == 2;
+
   // This lane's place in the reads below, to which (row, col) constants add.
   static __device__ __forceinline__ const T* row8_base(const T* t, int c, int g) { return t + c * PITCH + 8 * g; }
-  static __device__ __forceinline__ const T* row44_base(const T* t, int c, int g) { return t + c * PITCH + 4 * g; }
+  static __device__ __forceinline__ const T* row44_base(const T* t, int c, int g) {
+    return t + c * PITCH + (kPairs ? 8 : 4) * g;
+  }
+  static __device__ __forceinline__ const T* x8_base(const T* t, int c, int g) {
+    return kPairs ? t + c * PITCH + 16 * (g & 1) + 4 * (g >> 1) : row8_base(t, c, g);
+  }
   static __device__ __forceinline__ const T* col8_base(const T* t, int c, int g) {
     if constexpr (sizeof(T) == 4) return t + TOK_G * g * PITCH + c;
     else return t + (TOK_G * g + 2 * (c >> 2)) * PITCH + 4 * (c & 3);
@@ -82,16 +94,24 @@ struct Tile {
       return __builtin_bit_cast(typename Frag<T>::t, ld16(p));
     }
   }
-  // columns col + 4 g .. + 3 and col + 16 + 4 g .. + 3 of row + c: the order in
-  // which two accumulators hold 32 rows
+  // of X: columns col + 4 g .. + 3 and col + 16 + 4 g .. + 3 of row + c
   static __device__ __forceinline__ typename Frag<T>::t row44(const T* base, int row, int col) {
-    const T* p = base + row * PITCH + col;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (kPairs) {
+      return row8(base, row, col);
+    } else {
+      const T* p = base + row * PITCH + col;
       const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
       return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    } else {
-      const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 16);
+    }
+  }
+  // of X: columns col + 8 g .. + 7 of row + c
+  static __device__ __forceinline__ typename Frag<T>::t x8(const T* base, int row, int col) {
+    if constexpr (kPairs) {
+      const T* p = base + row * PITCH + col;
+      const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 8);
       return __builtin_bit_cast(typename Frag<T>::t, make_uint4(a.x, a.y, b.x, b.y));
+    } else {
+      return row8(base, row, col);
     }
   }
   // column col + c of rows row + TOK_G g + tok(j).  ds_read_b64_tr_b16 hands
@@ -128,11 +148,10 @@ struct Tile {
     }
   }
   static __device__ __forceinline__ const T* scores_base(const T* t, int c, int g) {
-    return sizeof(T) == 4 ? row44_base(t, c, g) : row8_base(t, c, g);
+    return row44_base(t, c, g);
   }
   static __device__ __forceinline__ typename Frag<T>::t scores(const T* base, int row, int col) {
-    if constexpr (sizeof(T) == 4) return row44(base, row, col);
-    else return row8(base, row, col);
+    return row44(base, row, col);
   }
 };
 
@@ -175,6 +194,19 @@ struct Stage {
     T* p = lds + threadIdx.x / L::CPR * L::PITCH + threadIdx.x % L::CPR * L::PER;
 #pragma unroll
     for (int i = 0; i < N; ++i) st16(p + i * RPT * L::PITCH, v[i]);
+  }
+  __device__ __forceinline__ void store_x(T* lds) const {
+    if constexpr (L::kPairs) {
+      const int c = threadIdx.x % L::CPR;  // the 4 columns 2 h and 2 h + 1 of 32, h = c % 4
+      T* p = lds + threadIdx.x / L::CPR * L::PITCH + 32 * (c >> 2) + 16 * (c & 1) + 4 * ((c >> 1) & 1);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        *reinterpret_cast<uint2*>(p + i * RPT * L::PITCH) = make_uint2(v[i].x, v[i].y);
+        *reinterpret_cast<uint2*>(p + i * RPT * L::PITCH + 8) = make_uint2(v[i].z, v[i].w);
+      }
+    } else {
+      store(lds);
+    }
   }
 };
 
@@ -269,6 +301,8 @@ struct WalkArgs {
   const float* log_decay;
   int64_t total;
   int batch, kv_heads, seg, slots;
+  int roles, members;     // walks in this launch; workgroups of one segment and K/V head over them
+  int start[kMaxRoles];   // first member of each role
   int terms;  // 16-bit operands that a weighted row of Z is split into (2 or 3)
 };
 
@@ -312,15 +346,18 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
   float* pow_p = pow + (OUT ? 2 * (C + 4) : 0);
   float* pow_i = pow_p + (OUT ? 2 * (C + 4) : 0);
 
-  const Role& r = a.role[blockIdx.y];
-  const int slices = (r.dz + DZ - 1) / DZ;
-  const int heads = OUT ? r.heads : a.kv_heads;
-  int item = blockIdx.x;
-  const int slice = item % slices;
-  item /= slices;
-  const int head = item % heads, slot = item / heads;
+  // Block b runs on XCD b % 8: the walks of one segment and K/V head, which
+  // read the same rows, are a group of blocks on one XCD (its L2 serves them).
+  const int place = blockIdx.x >> 3;
+  const int group = place / a.members * 8 + (blockIdx.x & 7);
+  int member = place % a.members, role = 0;
+  while (role + 1 < a.roles && member >= a.start[role + 1]) ++role;
+  member -= a.start[role];
+  const int kvh = group % a.kv_heads, slot = group / a.kv_heads;
   if (slot >= a.slots) return;
-  const int kvh = OUT ? head / r.x_group : head;
+  const Role& r = a.role[role];
+  const int slices = (r.dz + DZ - 1) / DZ;
+  const int slice = member % slices, head = OUT ? kvh * r.x_group + member / slices : kvh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int z0 = slice * DZ, zcols = min(DZ, r.dz - z0);
@@ -410,7 +447,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
       st16(ps + q * LP::PER, make_uint4(0u, 0u, 0u, 0u));
   }
   const float keep_whole = power(C);
-  const T *x8 = LX::row8_base(xs, c, g), *x44 = LX::row44_base(xs, c, g), *y8 = LX::row8_base(ys, c, g);
+  const T *x8 = LX::x8_base(xs, c, g), *x44 = LX::row44_base(xs, c, g), *y8 = LX::row8_base(ys, c, g);
   const T *yt = LX::col8_base(ys, c, g), *zt = LZ::col8_base(zs, c, g) + 16 * wave;
   const T* p8 = LP::scores_base(ps, c, g);
   T* pt = LP::score_base(ps, c, g);
@@ -429,7 +466,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
       sy.store(ys);
       sz.store(zs);
       if constexpr (OUT) {
-        if (yg == 0) sx.store(xs);
+        if (yg == 0) sx.store_x(xs);
       }
       __syncthreads();
       if (yg + 1 < y_group) fetch(ci, yg + 1);
@@ -442,7 +479,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
           const int strip = s0 + wave / WPS;
           F xf[DX / 32];
 #pragma unroll
-          for (int k = 0; k < DX / 32; ++k) xf[k] = LX::row8(x8, 16 * strip, 32 * k);
+          for (int k = 0; k < DX / 32; ++k) xf[k] = LX::x8(x8, 16 * strip, 32 * k);
 #pragma unroll
           for (int d = 0; d < ST; ++d) {
             if (d > strip || (WPS > 1 && d % WPS != wave % WPS)) continue;
@@ -794,13 +831,14 @@ size_t states_bytes(const Shape& s) {
 }
 
 template <typename T, int DX, int NW, bool OUT>
-int launch_walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
-  int64_t items = 0;
+int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
+  a.roles = roles;
+  a.members = 0;
   for (int i = 0; i < roles; ++i) {
-    const Role& r = a.role[i];
-    const int64_t n = (int64_t)a.slots * (OUT ? r.heads : a.kv_heads) * ((r.dz + 16 * NW - 1) / (16 * NW));
-    if (n > items) items = n;
+    a.start[i] = a.members;
+    a.members += (OUT ? a.role[i].x_group : 1) * ((a.role[i].dz + 16 * NW - 1) / (16 * NW));
   }
+  const int64_t items = ((int64_t)a.slots * a.kv_heads + 7) / 8 * 8 * a.members;
   if (items * 64 * NW > 0xffffffffll)
     return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
   constexpr size_t lds = walk_lds<T, DX, NW, OUT>();
@@ -811,7 +849,7 @@ int launch_walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (rc != hipSuccess) return set_error(SCREE_ERR_HIP, "%s: %s", fn, hipGetErrorString(rc));
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)items, roles), dim3(64 * NW), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)items), dim3(64 * NW), lds, stream, a);
   return check_launch(fn);
 }
 template <typename T, bool OUT, int DX>
