@@ -308,28 +308,29 @@ struct WalkArgs {
 
 template <typename T, int DX> constexpr int chunk_rows() { return sizeof(T) == 4 && DX == 256 ? 32 : 64; }
 
-template <typename T, int DX, int NW, bool OUT>
+template <typename T, int DX, int NW, int NT, bool OUT>
 constexpr size_t walk_lds() {
   constexpr int C = chunk_rows<T, DX>();
-  return sizeof(T) * (size_t)C * ((OUT ? 2 : 1) * Tile<T, DX>::PITCH + Tile<T, 16 * NW>::PITCH +
+  return sizeof(T) * (size_t)C * ((OUT ? 2 : 1) * Tile<T, DX>::PITCH + Tile<T, 16 * NT * NW>::PITCH +
                                   (OUT ? Tile<T, C>::PITCH : 0)) +
          sizeof(float) * (OUT ? 3 : 1) * 2 * (C + 4);
 }
 // Waves per SIMD that the registers are held to: as many as the LDS leaves room
-// for, four at most (128 registers).
-template <typename T, int DX, int NW, bool OUT>
+// for, but no more than the walk's registers allow without spills.
+template <typename T, int DX, int NW, int NT, bool OUT>
 constexpr int walk_waves() {
-  const int w = (int)(160 * 1024 / walk_lds<T, DX, NW, OUT>()) * NW / 4;
-  return w < 1 ? 1 : w > 4 ? 4 : w;
+  const int w = (int)(160 * 1024 / walk_lds<T, DX, NW, NT, OUT>()) * NW / 4;
+  constexpr int most = OUT ? 2 : 4;
+  return w < 1 ? 1 : w > most ? most : w;
 }
 
 // NW waves; wave w owns columns [16 w, 16 w + 16) of z, out and the state.
 // Two waves to a SIMD with 32 columns each (half the LDS reads, twice the
 // registers) ran 1.5x longer: what bounds the walk is waiting.
-template <typename T, int DX, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_walk_kernel(WalkArgs a) {
+template <typename T, int DX, int NW, int NT, bool OUT>
+__global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void lin_walk_kernel(WalkArgs a) {
   constexpr int C = chunk_rows<T, DX>();
-  constexpr int DZ = 16 * NW, THREADS = 64 * NW;
+  constexpr int CW = 16 * NT, DZ = CW * NW, THREADS = 64 * NW;
   constexpr int ST = C / 16;                   // strips of 16 rows
   constexpr int WPS = NW > ST ? NW / ST : 1;   // waves that share a strip of P
   typedef Tile<T, DX> LX;
@@ -419,8 +420,8 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
   }
   const int e = back ? 0 : 1;
 
-  // the state: element [m][i] is x-column 16 m + 4 g + i, z-column 16 wave + c
-  f32x4 st[DX / 16];
+  // the state: element [m][u][i] is x-column 16 m + 4 g + i, z-column CW wave + 16 u + c
+  f32x4 st[DX / 16][NT];
   const int64_t state_size = (int64_t)dx * r.dz;
   const bool whole = dx == DX && zcols == DZ;
   const float* in = nullptr;
@@ -429,16 +430,21 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
     else if (r.init) in = r.init + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
   }
   if (in) {
-    const float* p = in + 4 * g * r.s_x + (z0 + 16 * wave + c) * r.s_z;
-    const bool col = 16 * wave + c < zcols;
+    const float* p = in + 4 * g * r.s_x + (z0 + CW * wave + c) * r.s_z;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const bool col = CW * wave + 16 * u + c < zcols;
+#pragma unroll
+      for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st[m][u][i] = whole || (col && 16 * m + 4 * g + i < dx) ? p[(16 * m + i) * r.s_x + 16 * u * r.s_z] : 0.f;
+    }
+  } else {
 #pragma unroll
     for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st[m][i] = whole || (col && 16 * m + 4 * g + i < dx) ? p[(16 * m + i) * r.s_x] : 0.f;
-  } else {
-#pragma unroll
-    for (int m = 0; m < DX / 16; ++m) st[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < NT; ++u) st[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   if constexpr (OUT) {
@@ -448,7 +454,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
   }
   const float keep_whole = power(C);
   const T *x8 = LX::x8_base(xs, c, g), *x44 = LX::row44_base(xs, c, g), *y8 = LX::row8_base(ys, c, g);
-  const T *yt = LX::col8_base(ys, c, g), *zt = LZ::col8_base(zs, c, g) + 16 * wave;
+  const T *yt = LX::col8_base(ys, c, g), *zt = LZ::col8_base(zs, c, g) + CW * wave;
   const T* p8 = LP::scores_base(ps, c, g);
   T* pt = LP::score_base(ps, c, g);
   // weights of P's tiles d strips below the diagonal, lane (c, g) element i: row
@@ -459,7 +465,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
   // operands of a weighted row: an output state gets as many as fp32 has bits for
   const bool three = sizeof(T) == 2 && a.terms > 2 && (!OUT || sg.index == final);
 
-  f32x4 o[OUT ? ST : 1];
+  f32x4 o[NT][OUT ? ST : 1];
   for (int ci = 0; ci < chunks; ++ci) {
     const int n = chunk_rows_of(ci);
     for (int yg = 0; yg < y_group; ++yg) {
@@ -496,7 +502,9 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
         // they lie, in two 16-bit operands
         if (yg == 0) {
 #pragma unroll
-          for (int s = 0; s < ST; ++s) o[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < DX / 32; ++k) {
             // reads hoisted over several k would not fit the registers
@@ -504,90 +512,132 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
             F xf[ST];
 #pragma unroll
             for (int s = 0; s < ST; ++s) xf[s] = LX::row44(x44, 16 * s, 32 * k);
-            float f[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[i] = st[2 * k][i];
-              f[4 + i] = st[2 * k + 1][i];
+            for (int u = 0; u < NT; ++u) {
+              float f[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                f[i] = st[2 * k][u][i];
+                f[4 + i] = st[2 * k + 1][u][i];
+              }
+              if constexpr (sizeof(T) == 2) {
+                const F hi = take<T>(f);
+#pragma unroll
+                for (int s = 0; s < ST; ++s) mma(o[u][s], hi, xf[s]);
+              }
+              const F lo = to_frag<T>(f);
+#pragma unroll
+              for (int s = 0; s < ST; ++s) mma(o[u][s], lo, xf[s]);
             }
-            if constexpr (sizeof(T) == 2) {
-              const F hi = take<T>(f);
-#pragma unroll
-              for (int s = 0; s < ST; ++s) mma(o[s], hi, xf[s]);
-            }
-            const F lo = to_frag<T>(f);
-#pragma unroll
-            for (int s = 0; s < ST; ++s) mma(o[s], lo, xf[s]);
           }
 #pragma unroll
-          for (int s = 0; s < ST; ++s) o[s] *= wi[16 * s];
+          for (int s = 0; s < ST; ++s) {
+            const float w = wi[16 * s];
+#pragma unroll
+            for (int u = 0; u < NT; ++u) o[u][s] *= w;
+          }
         }
         __syncthreads();
       }
       if (yg == 0) {
         const float w = n == C ? keep_whole : power(n);
 #pragma unroll
-        for (int m = 0; m < DX / 16; ++m) st[m] *= w;
+        for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) st[m][u] *= w;
       }
       const float* wz = wz0 + n;
 #pragma unroll
       for (int kk = 0; kk < C / 32; ++kk) {
         __builtin_amdgcn_sched_barrier(0);
-        const F zf = LZ::col8(zt, 32 * kk, 0);
+        F zf[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) zf[u] = LZ::col8(zt, 32 * kk, 16 * u);
         if constexpr (OUT) {
 #pragma unroll
-          for (int s = 2 * kk; s < ST; ++s) mma(o[s], zf, LP::scores(p8, 16 * s, 32 * kk));
+          for (int s = 2 * kk; s < ST; ++s) {
+            const F pf = LP::scores(p8, 16 * s, 32 * kk);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) mma(o[u][s], zf[u], pf);
+          }
         }
         // Z weighted by lam^{n - e - i}, in two or three 16-bit operands
-        float rest[8];
+        float rest[NT][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) rest[j] = (float)zf[j] * wz[-(32 * kk + LX::tok(j))];
+        for (int j = 0; j < 8; ++j) {
+          const float w = wz[-(32 * kk + LX::tok(j))];
+#pragma unroll
+          for (int u = 0; u < NT; ++u) rest[u][j] = (float)zf[u][j] * w;
+        }
+        F hi[NT], lo[NT];
         if constexpr (sizeof(T) == 2) {
-          F hi = take<T>(rest);
+#pragma unroll
+          for (int u = 0; u < NT; ++u) hi[u] = take<T>(rest[u]);
           if (three) {
 #pragma unroll
-            for (int m = 0; m < DX / 16; ++m) mma(st[m], LX::col8(yt, 32 * kk, 16 * m), hi);
-            hi = take<T>(rest);
-          }
-          const F lo = to_frag<T>(rest);
+            for (int m = 0; m < DX / 16; ++m) {
+              const F yf = LX::col8(yt, 32 * kk, 16 * m);
 #pragma unroll
-          for (int m = 0; m < DX / 16; ++m) {
-            if (m % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-            const F yf = LX::col8(yt, 32 * kk, 16 * m);
-            mma(st[m], yf, hi);
-            mma(st[m], yf, lo);
-          }
-        } else {
-          const F zw = to_frag<T>(rest);
+              for (int u = 0; u < NT; ++u) mma(st[m][u], yf, hi[u]);
+            }
 #pragma unroll
-          for (int m = 0; m < DX / 16; ++m) mma(st[m], LX::col8(yt, 32 * kk, 16 * m), zw);
+            for (int u = 0; u < NT; ++u) hi[u] = take<T>(rest[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) lo[u] = to_frag<T>(rest[u]);
+#pragma unroll
+        for (int m = 0; m < DX / 16; ++m) {
+          if (m % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+          const F yf = LX::col8(yt, 32 * kk, 16 * m);
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) mma(st[m][u], yf, hi[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < NT; ++u) mma(st[m][u], yf, lo[u]);
         }
       }
       __syncthreads();
     }
     if constexpr (OUT) {
       const int64_t low = chunk_low(ci, n);
-      T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + head * r.o_head + z0 + 16 * wave;
+      T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + head * r.o_head + z0 + CW * wave;
       // row i of the chunk lies at i, or at n - 1 - i
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
           const int i = 16 * s + c;
-          if (i < n && 16 * wave + 4 * g < zcols)
-            *reinterpret_cast<float4*>(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + 4 * g) =
-                make_float4(o[s][0], o[s][1], o[s][2], o[s][3]);
+          T* dst = out + (int64_t)(back ? n - 1 - i : i) * r.o_row + 4 * g;
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+            if (i < n && CW * wave + 16 * u + 4 * g < zcols)
+              *reinterpret_cast<float4*>(dst + 16 * u) = make_float4(o[u][s][0], o[u][s][1], o[u][s][2], o[u][s][3]);
+        }
+      } else if constexpr (NT == 2) {
+        // a lane holds 4 columns of a row in either half of 32; exchanged between
+        // neighbouring groups, 8 in a row
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+          const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][0], o[0][s][1]), pack2<T>(o[1][s][0], o[1][s][1]),
+                                                           false, false);
+          const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[1][s][2], o[1][s][3]),
+                                                           false, false);
+          const int i = 16 * s + c, col = 16 * (g & 1) + 8 * (g >> 1);
+          if (i < n && CW * wave + col < zcols)
+            st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
         }
       } else {
         // a lane holds 4 columns of a row in every strip; exchanged between two
         // strips and neighbouring groups, 8 columns of a row in one of the two
 #pragma unroll
         for (int s = 0; s < ST; s += 2) {
-          const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[s][0], o[s][1]), pack2<T>(o[s + 1][0], o[s + 1][1]),
+          const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][0], o[0][s][1]), pack2<T>(o[0][s + 1][0], o[0][s + 1][1]),
                                                            false, false);
-          const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[s][2], o[s][3]), pack2<T>(o[s + 1][2], o[s + 1][3]),
+          const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[0][s + 1][2], o[0][s + 1][3]),
                                                            false, false);
           const int i = 16 * (s + (g & 1)) + c, col = 8 * (g >> 1);
-          if (i < n && 16 * wave + col < zcols)
+          if (i < n && CW * wave + col < zcols)
             st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
         }
       }
@@ -606,13 +656,16 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, OUT>())) void lin_w
   // would take its registers
   int g_ = g, c_ = c;
   asm volatile("" : "+v"(g_), "+v"(c_));
-  to += 4 * g_ * r.s_x + (z0 + 16 * wave + c_) * r.s_z;
-  const bool col = 16 * wave + c_ < zcols;
+  to += 4 * g_ * r.s_x + (z0 + CW * wave + c_) * r.s_z;
 #pragma unroll
-  for (int m = 0; m < DX / 16; ++m)
+  for (int u = 0; u < NT; ++u) {
+    const bool col = CW * wave + 16 * u + c_ < zcols;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (whole || (col && 16 * m + 4 * g_ + i < dx)) to[(16 * m + i) * r.s_x] = st[m][i];
+    for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (whole || (col && 16 * m + 4 * g_ + i < dx)) to[(16 * m + i) * r.s_x + 16 * u * r.s_z] = st[m][u][i];
+  }
 }
 
 // The segments' own states become the states that come into them: along each
@@ -830,20 +883,20 @@ size_t states_bytes(const Shape& s) {
   return (size_t)slot_count(s.total, s.batch, seg) * s.kv_heads * s.dk * s.dv * sizeof(float);
 }
 
-template <typename T, int DX, int NW, bool OUT>
+template <typename T, int DX, int NW, int NT, bool OUT>
 int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
   a.roles = roles;
   a.members = 0;
   for (int i = 0; i < roles; ++i) {
     a.start[i] = a.members;
-    a.members += (OUT ? a.role[i].x_group : 1) * ((a.role[i].dz + 16 * NW - 1) / (16 * NW));
+    a.members += (OUT ? a.role[i].x_group : 1) * ((a.role[i].dz + 16 * NT * NW - 1) / (16 * NT * NW));
   }
   const int64_t items = ((int64_t)a.slots * a.kv_heads + 7) / 8 * 8 * a.members;
   if (items * 64 * NW > 0xffffffffll)
     return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
-  constexpr size_t lds = walk_lds<T, DX, NW, OUT>();
+  constexpr size_t lds = walk_lds<T, DX, NW, NT, OUT>();
   static_assert(lds <= 160 * 1024, "LDS of a CU");
-  auto kernel = lin_walk_kernel<T, DX, NW, OUT>;
+  auto kernel = lin_walk_kernel<T, DX, NW, NT, OUT>;
   if (lds > 64 * 1024) {
     const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -854,13 +907,22 @@ int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
 }
 template <typename T, bool OUT, int DX>
 int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
-  // waves enough for z's columns, and for the rows staged in their registers
   const int dz = a.role[0].dz;
-  if constexpr (DX <= 64)
-    if (dz <= 32) return launch_walk<T, DX, 2, OUT>(fn, a, roles, stream);
-  if constexpr (DX <= 128)
-    if (DX <= 32 || dz <= 64) return launch_walk<T, DX, 4, OUT>(fn, a, roles, stream);
-  if constexpr (DX > 32) return launch_walk<T, DX, 8, OUT>(fn, a, roles, stream);
+#define WALK(NW, NT) return launch_walk<T, DX, NW, NT, OUT>(fn, a, roles, stream)
+  if constexpr (OUT && sizeof(T) == 2 && DX <= 128) {
+    if constexpr (DX <= 32)
+      if (dz <= 32) WALK(1, 2);
+    if constexpr (DX <= 64)
+      if (dz <= 64) WALK(2, 2);
+    WALK(4, 2);
+  } else {
+    if constexpr (DX <= 64)
+      if (dz <= 32) WALK(2, 1);
+    if constexpr (DX <= 128)
+      if (DX <= 32 || dz <= 64) WALK(4, 1);
+    if constexpr (DX > 32) WALK(8, 1);
+  }
+#undef WALK
 }
 // One launch for `roles` walks of equal dims.
 template <typename T, bool OUT>
