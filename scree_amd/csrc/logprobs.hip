@@ -97,18 +97,48 @@ __device__ __forceinline__ bool ahead(float av, int ai, float bv, int bi) {
 __device__ __forceinline__ float lane_f(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
-// Insert the wave-uniform (v, i): the entries behind it move down one lane.
+// Insert the wave-uniform (v, i): the entries behind it move down one lane
+// (wave_shr:1).  The bound to beat stays while entry top_k - 1 is unused.
 __device__ __forceinline__ void insert(TopList& l, float v, int i, int top_k) {
   const int lane = threadIdx.x & 63;
   const int pos = __popcll(__ballot(ahead(l.v, l.i, v, i)));
-  const float pv = __shfl_up(l.v, 1);
-  const int pi = __shfl_up(l.i, 1);
+  const int lv = __builtin_bit_cast(int, l.v);
+  const float pv = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(lv, lv, 0x138, 0xf, 0xf, false));
+  const int pi = __builtin_amdgcn_update_dpp(l.i, l.i, 0x138, 0xf, 0xf, false);
   if (lane >= pos) {
     l.v = lane == pos ? v : pv;
     l.i = lane == pos ? i : pi;
   }
-  l.last_v = lane_f(l.v, top_k - 1);
-  l.last_i = __builtin_amdgcn_readlane(l.i, top_k - 1);
+  const int last_i = __builtin_amdgcn_readlane(l.i, top_k - 1);
+  if (last_i != 0x7fffffff) {
+    l.last_v = lane_f(l.v, top_k - 1);
+    l.last_i = last_i;
+  }
+}
+// A first bound for an empty list: with the largest elements that N groups of
+// 64 lanes hold, at least top_k elements reach the top_k-th largest of those.
+// Found bit by bit in the upper half of the ordered bits, so at most 2^-7 of
+// its value below; the list then takes few more than top_k elements instead of
+// every new largest (16 rows x 128,000 with 20 alternatives: 54 -> 27 us).
+template <int N>
+__device__ __forceinline__ void seed(TopList& l, const float (&mx)[N], int top_k) {
+  uint32_t key[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, mx[n]);
+    key[n] = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+  }
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = t | (1u << bit);
+    int count = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) count += __popcll(__ballot(key[n] >= c));
+    if (count >= top_k) t = c;
+  }
+  const float v = __builtin_bit_cast(float, t & 0x80000000u ? t ^ 0x80000000u : ~t);
+  l.last_v = v == v ? v : -__builtin_inff();  // the bits below -inf are NaN
 }
 // Offer every lane's (v, i); lanes with nothing to offer pass NaN.
 __device__ __forceinline__ void offer(TopList& l, float v, int i, int top_k) {
@@ -172,8 +202,11 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
   TopList l;
   if constexpr (TOP) l.init();
   const int whole = c0 + (c1 - c0) / VEC * VEC;
-  // trips are uniform over a wave (its list needs every lane)
-  for (int base = c0 + wave * 64 * VEC; base < whole; base += U * kLpThreads * VEC) {
+  __shared__ float lane_max[TOP ? kLpThreads : 1];
+  // trips are uniform over a wave (its list needs every lane), the first over
+  // the workgroup (its lanes' maxima bound the lists)
+  int base = c0 + wave * 64 * VEC;
+  do {
     uint4 v[U];
     bool have[U];
 #pragma unroll
@@ -182,18 +215,29 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
       have[u] = c < whole;
       if (have[u]) v[u] = ld16_elem(x + c);
     }
-    float hi = a.m;
+    float mx[U], hi = a.m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float mx = -__builtin_inff();
+      mx[u] = -__builtin_inff();
       if (have[u]) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, elem<T>(v[u], e));
+        for (int e = 0; e < VEC; ++e) mx[u] = fmaxf(mx[u], elem<T>(v[u], e));
       }
-      hi = fmaxf(hi, mx);
-      if constexpr (TOP) {
+      hi = fmaxf(hi, mx[u]);
+    }
+    if constexpr (TOP) {
+      if (base < c0 + kLpThreads * VEC) {
+        lane_max[tid] = hi;
+        __syncthreads();
+        float mxs[kLpWaves];
+#pragma unroll
+        for (int w = 0; w < kLpWaves; ++w) mxs[w] = lane_max[64 * w + lane];
+        seed(l, mxs, top_k);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
         const int c = base + u * kLpThreads * VEC + lane * VEC;
-        if (__ballot(have[u] && mx >= l.last_v)) {
+        if (__ballot(have[u] && mx[u] >= l.last_v)) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
             offer(l, have[u] ? elem<T>(v[u], e) : __builtin_nanf(""), c + e, top_k);
@@ -214,7 +258,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
         a.t = fmaf(p, fmaxf(d, kLowest), a.t);
       }
     }
-  }
+    base += U * kLpThreads * VEC;
+  } while (base < whole);
   if (wave == 0) {  // the last columns, fewer than a vector
     const bool have = whole + lane < c1;
     const float f = have ? to_f32(x[whole + lane]) : -__builtin_inff();
@@ -280,10 +325,19 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(
   if (top_k) {
     const float2* pt = part_top + row * parts * top_k;
     const int n = parts * top_k;
-    for (int base = 0; base < n; base += 64) {
-      const bool have = base + lane < n;
-      const float2 c = have ? pt[base + lane] : make_float2(__builtin_nanf(""), 0.f);
-      offer(l, c.x, __builtin_bit_cast(int, c.y), top_k);
+    constexpr int R = 12;  // a lane's candidates per turn, their loads issued together
+    for (int base = 0; base < n; base += 64 * R) {
+      float2 c[R];
+      float mx[1] = {-__builtin_inff()};
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int at = base + 64 * i + lane;
+        c[i] = at < n ? pt[at] : make_float2(__builtin_nanf(""), 0.f);
+        mx[0] = fmaxf(mx[0], c[i].x);
+      }
+      if (base == 0) seed(l, mx, top_k);
+#pragma unroll
+      for (int i = 0; i < R; ++i) offer(l, c[i].x, __builtin_bit_cast(int, c[i].y), top_k);
     }
   }
   const int64_t target = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row]
