@@ -311,9 +311,10 @@ int scree_varlen_softmax_bwd(const void* y, const void* dy, void* dx, const int3
  * past the last sequence are left as they were.  No counterpart in the
  * reference. */
 
-/* Bytes of workspace for the forward (or the backward): the fp32 states
- * between the segments that long sequences are walked in; 0 when no sequence
- * can have two. */
+/* Bytes of workspace for the forward: the fp32 states between the segments
+ * that long sequences are walked in; 0 when no sequence can have two.  The
+ * backward needs as many when it is given the forward's workspace, else
+ * (`backward` nonzero) twice that. */
 size_t scree_linear_attn_workspace_bytes(int batch, int64_t total_tokens, int heads, int kv_heads,
                                          int k_dim, int v_dim, int backward);
 
@@ -328,14 +329,18 @@ int scree_linear_attn_fwd(const void* q, const void* k, const void* v, const flo
 /* dq, dk, dv (and dinitial_state unless NULL) from dout, the final state's
  * gradient (may be NULL: zero) and the forward's inputs; dk and dv sum over
  * each group's query heads, without atomics.  Rows past the last sequence
- * become zeros.  strides[14] = {dout, q, k, v, dq, dk, dv} x {row, head}. */
+ * become zeros.  `fwd_workspace` may be the workspace of the forward call with
+ * the same q, k, v, log_decay, initial_state, offsets and sizes, left as that
+ * call wrote it (it is only read), or NULL.  `scale` must be finite and not
+ * zero.  In fp16 the rounded scores (scale * q.k here and in the forward,
+ * scale * do.v) overflow past 65504.  strides[14] = {dout, q, k, v, dq, dk, dv} x {row, head}. */
 int scree_linear_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
                           const float* log_decay, void* dq, void* dk, void* dv,
                           const float* initial_state, const float* dfinal_state,
-                          float* dinitial_state, const int32_t* cu_seqlens, int batch,
-                          int64_t total_tokens, int heads, int kv_heads, int k_dim, int v_dim,
-                          const int64_t* strides, float scale, int dtype, void* workspace,
-                          size_t workspace_bytes, void* stream);
+                          float* dinitial_state, const void* fwd_workspace,
+                          const int32_t* cu_seqlens, int batch, int64_t total_tokens, int heads,
+                          int kv_heads, int k_dim, int v_dim, const int64_t* strides, float scale,
+                          int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* One token for each of `rows` sequences: state_out = lam state + k v^T and
  * o = scale * state_out^T q; state_out may be `state` (in place).

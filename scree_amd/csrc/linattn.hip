@@ -286,19 +286,20 @@ struct Role {
   float* last;         // (batch, kv_heads, state): the state that goes out, may be null
   float* seg_state;    // (slots, kv_heads, state)
   int64_t s_x, s_z;    // the state's strides along x's and z's axes
-  int heads;           // of x and out
   int x_group;         // heads of x per K/V head
+  int x_loop;          // of which a workgroup takes this many, one after the other in every chunk
   int y_group;         // heads of y and z per K/V head, summed
   int dx, dz;
   int reverse;
   int zero_tail;       // rows past the last sequence become zeros (gradients)
-  float p_mul, i_mul, z_mul;  // factors of P, of the state's share, of Z in the state's update
+  float in_mul, out_mul;  // the state's factors on its way in and out
 };
 constexpr int kMaxRoles = 3;
 struct WalkArgs {
   Role role[kMaxRoles];
   const int32_t* cu;
   const float* log_decay;
+  float scale;
   int64_t total;
   int batch, kv_heads, seg, slots;
   int roles, members;     // walks in this launch; workgroups of one segment and K/V head over them
@@ -313,7 +314,7 @@ constexpr size_t walk_lds() {
   constexpr int C = chunk_rows<T, DX>();
   return sizeof(T) * (size_t)C * ((OUT ? 2 : 1) * Tile<T, DX>::PITCH + Tile<T, 16 * NT * NW>::PITCH +
                                   (OUT ? Tile<T, C>::PITCH : 0)) +
-         sizeof(float) * (OUT ? 3 : 1) * 2 * (C + 4);
+         sizeof(float) * (OUT ? 2 : 1) * 2 * (C + 4);
 }
 // Waves per SIMD that the registers are held to: as many as the LDS leaves room
 // for, but no more than the walk's registers allow without spills.
@@ -327,7 +328,8 @@ constexpr int walk_waves() {
 // NW waves; wave w owns columns [16 w, 16 w + 16) of z, out and the state.
 // Two waves to a SIMD with 32 columns each (half the LDS reads, twice the
 // registers) ran 1.5x longer: what bounds the walk is waiting.
-template <typename T, int DX, int NW, int NT, bool OUT>
+// XLOOP: x's heads of a group in turn (x_loop > 1).
+template <typename T, int DX, int NW, int NT, bool OUT, bool XLOOP>
 __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void lin_walk_kernel(WalkArgs a) {
   constexpr int C = chunk_rows<T, DX>();
   constexpr int CW = 16 * NT, DZ = CW * NW, THREADS = 64 * NW;
@@ -342,10 +344,9 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   T* zs = ys + C * LX::PITCH;
   T* xs = zs + C * LZ::PITCH;
   T* ps = xs + (OUT ? C * LX::PITCH : 0);
-  // lam^n, -C <= n <= C, 0 for n < 0: times z_mul, p_mul and i_mul
+  // lam^n, -C <= n <= C, 0 for n < 0, and the same times scale
   float* pow = reinterpret_cast<float*>(ps + (OUT ? C * LP::PITCH : 0)) + C;
-  float* pow_p = pow + (OUT ? 2 * (C + 4) : 0);
-  float* pow_i = pow_p + (OUT ? 2 * (C + 4) : 0);
+  float* pow_s = pow + (OUT ? 2 * (C + 4) : 0);
 
   // Block b runs on XCD b % 8: the walks of one segment and K/V head, which
   // read the same rows, are a group of blocks on one XCD (its L2 serves them).
@@ -358,7 +359,8 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   if (slot >= a.slots) return;
   const Role& r = a.role[role];
   const int slices = (r.dz + DZ - 1) / DZ;
-  const int slice = member % slices, head = OUT ? kvh * r.x_group + member / slices : kvh;
+  const int slice = member % slices, x_loop = XLOOP ? r.x_loop : 1;
+  const int head = OUT ? kvh * r.x_group + member / slices * x_loop : kvh;  // the first of x's
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int z0 = slice * DZ, zcols = min(DZ, r.dz - z0);
@@ -366,13 +368,15 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   if constexpr (OUT) {
     // rows behind the last sequence: the last slot's workgroups
     if (r.zero_tail && slot == a.slots - 1) {
-      T* out = static_cast<T*>(r.out) + head * r.o_head + z0;
       const int per = zcols / 8;
       const int64_t tail = offset_at(a.cu, a.batch, a.total);
-      for (int64_t q = threadIdx.x; q < (a.total - tail) * per; q += THREADS) {
-        T* p = out + (tail + q / per) * r.o_row + (int)(q % per) * 8;
-        st16(p, make_uint4(0u, 0u, 0u, 0u));
-        if constexpr (sizeof(T) == 4) st16(p + 4, make_uint4(0u, 0u, 0u, 0u));
+      for (int h = 0; h < x_loop; ++h) {
+        T* out = static_cast<T*>(r.out) + (head + h) * r.o_head + z0;
+        for (int64_t q = threadIdx.x; q < (a.total - tail) * per; q += THREADS) {
+          T* p = out + (tail + q / per) * r.o_row + (int)(q % per) * 8;
+          st16(p, make_uint4(0u, 0u, 0u, 0u));
+          if constexpr (sizeof(T) == 4) st16(p + 4, make_uint4(0u, 0u, 0u, 0u));
+        }
       }
     }
   }
@@ -388,35 +392,37 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   const T* x = static_cast<const T*>(r.x) + (OUT ? sg.row0 * r.x_row + head * r.x_head : 0);
   const T* y = static_cast<const T*>(r.y) + sg.row0 * r.y_row + (int64_t)kvh * y_group * r.y_head;
   const T* z = static_cast<const T*>(r.z) + sg.row0 * r.z_row + (int64_t)kvh * y_group * r.z_head + z0;
-  const int64_t x_row = r.x_row, y_row = r.y_row, z_row = r.z_row, y_head = r.y_head, z_head = r.z_head;
+  const int64_t x_row = r.x_row, x_head = r.x_head, y_row = r.y_row, z_row = r.z_row, y_head = r.y_head, z_head = r.z_head;
   Stage<T, DX, C, THREADS> sx, sy;
   Stage<T, DZ, C, THREADS> sz;
   // chunk ci has n rows from row `low`: the walk's order from the segment's
   // start, or from its end
   auto chunk_rows_of = [&](int ci) { return min(C, rows - ci * C); };
   auto chunk_low = [&](int ci, int n) { return (int64_t)(back ? rows - ci * C - n : ci * C); };
-  auto fetch = [&](int ci, int yg) {
-    const int n = chunk_rows_of(ci);
+  // A chunk takes `turns` turns: over x's heads, which share Y and Z and the
+  // state that came in, or over y's and z's, which sum into X's output.
+  constexpr bool over_x = XLOOP;
+  const int turns = over_x ? x_loop : y_group, chunks = (rows + C - 1) / C;
+  // what chunk ci, turn `turn` brings (nothing past the last chunk: no rows)
+  auto fetch = [&](int ci, int turn) {
+    const int n = ci < chunks ? chunk_rows_of(ci) : 0;
     const int64_t low = chunk_low(ci, n);
-    sy.load(y + low * y_row + yg * y_head, y_row, n, dx, back);
-    sz.load(z + low * z_row + yg * z_head, z_row, n, zcols, back);
-    if constexpr (OUT) {
-      if (yg == 0) sx.load(x + low * x_row, x_row, n, dx, back);
-    }
+    const int64_t yz = over_x ? 0 : turn;
+    const int n_yz = over_x && turn ? 0 : n;
+    sy.load(y + low * y_row + yz * y_head, y_row, n_yz, dx, back);
+    sz.load(z + low * z_row + yz * z_head, z_row, n_yz, zcols, back);
+    if constexpr (OUT)
+      sx.load(x + low * x_row + (over_x ? turn : 0) * x_head, x_row, over_x || !turn ? n : 0, dx, back);
   };
-  const int chunks = (rows + C - 1) / C;
-  if (chunks) fetch(0, 0);
+  fetch(0, 0);
 
   const float g2 = a.log_decay[kvh] * 1.4426950408889634f;
   // lam^n; lam^0 is 1 also for a decay of -inf
   auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)n); };
   for (int n = (int)threadIdx.x - C; n <= C; n += THREADS) {
     const float w = n < 0 ? 0.f : power(n);
-    pow[n] = w * r.z_mul;
-    if constexpr (OUT) {
-      pow_p[n] = w * r.p_mul;
-      pow_i[n] = w * r.i_mul;
-    }
+    pow[n] = w;
+    if constexpr (OUT) pow_s[n] = w * a.scale;
   }
   const int e = back ? 0 : 1;
 
@@ -425,8 +431,9 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   const int64_t state_size = (int64_t)dx * r.dz;
   const bool whole = dx == DX && zcols == DZ;
   const float* in = nullptr;
+  float in_mul = r.in_mul;  // a segment's state has it already
   if constexpr (OUT) {
-    if (sg.index != first) in = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
+    if (sg.index != first) in_mul = 1.f, in = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
     else if (r.init) in = r.init + ((int64_t)sg.seq * a.kv_heads + kvh) * state_size;
   }
   if (in) {
@@ -438,7 +445,8 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
       for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          st[m][u][i] = whole || (col && 16 * m + 4 * g + i < dx) ? p[(16 * m + i) * r.s_x + 16 * u * r.s_z] : 0.f;
+          st[m][u][i] =
+              whole || (col && 16 * m + 4 * g + i < dx) ? p[(16 * m + i) * r.s_x + 16 * u * r.s_z] * in_mul : 0.f;
     }
   } else {
 #pragma unroll
@@ -460,7 +468,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   // weights of P's tiles d strips below the diagonal, lane (c, g) element i: row
   // t = c, column s = 4 g + i, lam^{16 d + c - 4 g - i}; of the state's share,
   // row c of strip s, lam^{16 s + c + e}
-  const float *wp = pow_p + c - 4 * g, *wi = pow_i + c + e;
+  const float *wp = pow_s + c - 4 * g, *wi = pow_s + c + e;
   const float* wz0 = pow - e - LX::TOK_G * g;
   // operands of a weighted row: an output state gets as many as fp32 has bits for
   const bool three = sizeof(T) == 2 && a.terms > 2 && (!OUT || sg.index == final);
@@ -468,15 +476,17 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   f32x4 o[NT][OUT ? ST : 1];
   for (int ci = 0; ci < chunks; ++ci) {
     const int n = chunk_rows_of(ci);
-    for (int yg = 0; yg < y_group; ++yg) {
-      sy.store(ys);
-      sz.store(zs);
+    for (int turn = 0; turn < turns; ++turn) {
+      const bool last_turn = turn == turns - 1;
+      if (!over_x || turn == 0) {
+        sy.store(ys);
+        sz.store(zs);
+      }
       if constexpr (OUT) {
-        if (yg == 0) sx.store_x(xs);
+        if (over_x || turn == 0) sx.store_x(xs);
       }
       __syncthreads();
-      if (yg + 1 < y_group) fetch(ci, yg + 1);
-      else if (ci + 1 < chunks) fetch(ci + 1, 0);
+      fetch(last_turn ? ci + 1 : ci, last_turn ? 0 : turn + 1);
 
       if constexpr (OUT) {
         // P, a strip of 16 rows to WPS waves (every WPS-th tile each), rounded to T
@@ -500,7 +510,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
         }
         // out^T = (X A)^T lam^{i+e}: the state's accumulators are its operand as
         // they lie, in two 16-bit operands
-        if (yg == 0) {
+        if (over_x || turn == 0) {
 #pragma unroll
           for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -539,7 +549,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
         }
         __syncthreads();
       }
-      if (yg == 0) {
+      if (over_x ? last_turn : turn == 0) {
         const float w = n == C ? keep_whole : power(n);
 #pragma unroll
         for (int m = 0; m < DX / 16; ++m)
@@ -561,6 +571,8 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
             for (int u = 0; u < NT; ++u) mma(o[u][s], zf[u], pf);
           }
         }
+        if constexpr (over_x)
+          if (!last_turn) continue;
         // Z weighted by lam^{n - e - i}, in two or three 16-bit operands
         float rest[NT][8];
 #pragma unroll
@@ -599,52 +611,54 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
         }
       }
       __syncthreads();
-    }
-    if constexpr (OUT) {
-      const int64_t low = chunk_low(ci, n);
-      T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + head * r.o_head + z0 + CW * wave;
-      // row i of the chunk lies at i, or at n - 1 - i
-      if constexpr (sizeof(T) == 4) {
+      if constexpr (OUT) {
+        if (!over_x && !last_turn) continue;
+        const int64_t low = chunk_low(ci, n);
+        T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + (head + (over_x ? turn : 0)) * r.o_head + z0 + CW * wave;
+        // row i of the chunk lies at i, or at n - 1 - i
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int s = 0; s < ST; ++s) {
-          const int i = 16 * s + c;
-          T* dst = out + (int64_t)(back ? n - 1 - i : i) * r.o_row + 4 * g;
+          for (int s = 0; s < ST; ++s) {
+            const int i = 16 * s + c;
+            T* dst = out + (int64_t)(back ? n - 1 - i : i) * r.o_row + 4 * g;
 #pragma unroll
-          for (int u = 0; u < NT; ++u)
-            if (i < n && CW * wave + 16 * u + 4 * g < zcols)
-              *reinterpret_cast<float4*>(dst + 16 * u) = make_float4(o[u][s][0], o[u][s][1], o[u][s][2], o[u][s][3]);
-        }
-      } else if constexpr (NT == 2) {
-        // a lane holds 4 columns of a row in either half of 32; exchanged between
-        // neighbouring groups, 8 in a row
+            for (int u = 0; u < NT; ++u)
+              if (i < n && CW * wave + 16 * u + 4 * g < zcols)
+                *reinterpret_cast<float4*>(dst + 16 * u) = make_float4(o[u][s][0], o[u][s][1], o[u][s][2], o[u][s][3]);
+          }
+        } else if constexpr (NT == 2) {
+          // a lane holds 4 columns of a row in either half of 32; exchanged between
+          // neighbouring groups, 8 in a row
 #pragma unroll
-        for (int s = 0; s < ST; ++s) {
-          const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][0], o[0][s][1]), pack2<T>(o[1][s][0], o[1][s][1]),
-                                                           false, false);
-          const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[1][s][2], o[1][s][3]),
-                                                           false, false);
-          const int i = 16 * s + c, col = 16 * (g & 1) + 8 * (g >> 1);
-          if (i < n && CW * wave + col < zcols)
-            st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
-        }
-      } else {
-        // a lane holds 4 columns of a row in every strip; exchanged between two
-        // strips and neighbouring groups, 8 columns of a row in one of the two
+          for (int s = 0; s < ST; ++s) {
+            const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][0], o[0][s][1]), pack2<T>(o[1][s][0], o[1][s][1]),
+                                                             false, false);
+            const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[1][s][2], o[1][s][3]),
+                                                             false, false);
+            const int i = 16 * s + c, col = 16 * (g & 1) + 8 * (g >> 1);
+            if (i < n && CW * wave + col < zcols)
+              st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
+          }
+        } else {
+          // a lane holds 4 columns of a row in every strip; exchanged between two
+          // strips and neighbouring groups, 8 columns of a row in one of the two
 #pragma unroll
-        for (int s = 0; s < ST; s += 2) {
-          const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][0], o[0][s][1]), pack2<T>(o[0][s + 1][0], o[0][s + 1][1]),
-                                                           false, false);
-          const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[0][s + 1][2], o[0][s + 1][3]),
-                                                           false, false);
-          const int i = 16 * (s + (g & 1)) + c, col = 8 * (g >> 1);
-          if (i < n && CW * wave + col < zcols)
-            st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
+          for (int s = 0; s < ST; s += 2) {
+            const auto e0 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][0], o[0][s][1]), pack2<T>(o[0][s + 1][0], o[0][s + 1][1]),
+                                                             false, false);
+            const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[0][s + 1][2], o[0][s + 1][3]),
+                                                             false, false);
+            const int i = 16 * (s + (g & 1)) + c, col = 8 * (g >> 1);
+            if (i < n && CW * wave + col < zcols)
+              st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
+          }
         }
       }
     }
   }
 
   float* to = nullptr;
+  const float out_mul = OUT ? r.out_mul : 1.f;
   if constexpr (!OUT) {
     to = r.seg_state + ((int64_t)slot * a.kv_heads + kvh) * state_size;
   } else {
@@ -664,7 +678,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
     for (int m = 0; m < DX / 16; ++m)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (whole || (col && 16 * m + 4 * g_ + i < dx)) to[(16 * m + i) * r.s_x + 16 * u * r.s_z] = st[m][u][i];
+        if (whole || (col && 16 * m + 4 * g_ + i < dx)) to[(16 * m + i) * r.s_x + 16 * u * r.s_z] = st[m][u][i] * out_mul;
   }
 }
 
@@ -685,7 +699,13 @@ __global__ __launch_bounds__(kChainThreads) void lin_chain_kernel(WalkArgs a) {
   const int slot0 = (int)(s0 / a.seg) + seq;
   const float g2 = a.log_decay[kvh] * 1.4426950408889634f;
   float4 cur = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (r.init) cur = *reinterpret_cast<const float4*>(r.init + ((int64_t)seq * a.kv_heads + kvh) * state + 4 * q);
+  if (r.init) {
+    cur = *reinterpret_cast<const float4*>(r.init + ((int64_t)seq * a.kv_heads + kvh) * state + 4 * q);
+    cur.x *= r.in_mul;
+    cur.y *= r.in_mul;
+    cur.z *= r.in_mul;
+    cur.w *= r.in_mul;
+  }
   constexpr int U = 8;
   for (int j0 = 0; j0 < count; j0 += U) {
     float4 own[U];
@@ -821,8 +841,8 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 constexpr int64_t kLinFill = 1024;
 constexpr int kLinMinSeg = 256, kLinMaxSeg = 2048;
 
-inline int segment_tokens(int64_t total, int heads) {
-  int64_t m = (total * heads / kLinFill + 63) / 64 * 64;
+inline int segment_tokens(int64_t total, int kv_heads) {
+  int64_t m = (total * kv_heads / kLinFill + 63) / 64 * 64;
   if (m < kLinMinSeg) m = kLinMinSeg;
   if (m > kLinMaxSeg) m = kLinMaxSeg;
   return (int)m;
@@ -878,25 +898,25 @@ int check_states(const char* fn, const void* const* p, int n) {
 
 // Bytes of one set of segment states (0: no sequence can have two segments).
 size_t states_bytes(const Shape& s) {
-  const int seg = segment_tokens(s.total, s.heads);
+  const int seg = segment_tokens(s.total, s.kv_heads);
   if (s.total <= seg) return 0;
   return (size_t)slot_count(s.total, s.batch, seg) * s.kv_heads * s.dk * s.dv * sizeof(float);
 }
 
-template <typename T, int DX, int NW, int NT, bool OUT>
+template <typename T, int DX, int NW, int NT, bool OUT, bool XLOOP>
 int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
   a.roles = roles;
   a.members = 0;
   for (int i = 0; i < roles; ++i) {
     a.start[i] = a.members;
-    a.members += (OUT ? a.role[i].x_group : 1) * ((a.role[i].dz + 16 * NT * NW - 1) / (16 * NT * NW));
+    a.members += (OUT ? a.role[i].x_group / a.role[i].x_loop : 1) * ((a.role[i].dz + 16 * NT * NW - 1) / (16 * NT * NW));
   }
   const int64_t items = ((int64_t)a.slots * a.kv_heads + 7) / 8 * 8 * a.members;
   if (items * 64 * NW > 0xffffffffll)
     return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
   constexpr size_t lds = walk_lds<T, DX, NW, NT, OUT>();
   static_assert(lds <= 160 * 1024, "LDS of a CU");
-  auto kernel = lin_walk_kernel<T, DX, NW, NT, OUT>;
+  auto kernel = lin_walk_kernel<T, DX, NW, NT, OUT, XLOOP>;
   if (lds > 64 * 1024) {
     const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -905,10 +925,10 @@ int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)items), dim3(64 * NW), lds, stream, a);
   return check_launch(fn);
 }
-template <typename T, bool OUT, int DX>
+template <typename T, bool OUT, bool XLOOP, int DX>
 int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
   const int dz = a.role[0].dz;
-#define WALK(NW, NT) return launch_walk<T, DX, NW, NT, OUT>(fn, a, roles, stream)
+#define WALK(NW, NT) return launch_walk<T, DX, NW, NT, OUT, XLOOP>(fn, a, roles, stream)
   if constexpr (OUT && sizeof(T) == 2 && DX <= 128) {
     if constexpr (DX <= 32)
       if (dz <= 32) WALK(1, 2);
@@ -924,18 +944,22 @@ int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
   }
 #undef WALK
 }
-// One launch for `roles` walks of equal dims.
-template <typename T, bool OUT>
+// One launch for `roles` walks of equal dims, all with x_loop > 1 or none.
+template <typename T, bool OUT, bool XLOOP>
 int walk(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
   const int dx = a.role[0].dx;
-  if (dx <= 32) return walk_z<T, OUT, 32>(fn, a, roles, stream);
-  if (dx <= 64) return walk_z<T, OUT, 64>(fn, a, roles, stream);
-  if (dx <= 128) return walk_z<T, OUT, 128>(fn, a, roles, stream);
-  return walk_z<T, OUT, 256>(fn, a, roles, stream);
+  if (dx <= 32) return walk_z<T, OUT, XLOOP, 32>(fn, a, roles, stream);
+  if (dx <= 64) return walk_z<T, OUT, XLOOP, 64>(fn, a, roles, stream);
+  if (dx <= 128) return walk_z<T, OUT, XLOOP, 128>(fn, a, roles, stream);
+  return walk_z<T, OUT, XLOOP, 256>(fn, a, roles, stream);
+}
+template <typename T>
+int walk_out(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
+  return a.role[0].x_loop > 1 ? walk<T, true, true>(fn, a, roles, stream) : walk<T, true, false>(fn, a, roles, stream);
 }
 template <typename T>
 int segment_states(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
-  if (int rc = walk<T, false>(fn, a, roles, stream)) return rc;
+  if (int rc = walk<T, false, false>(fn, a, roles, stream)) return rc;
   const int64_t state = (int64_t)a.role[0].dx * a.role[0].dz;
   const int64_t per = (state / 4 + kChainThreads - 1) / kChainThreads;
   const int64_t items = per * a.kv_heads * a.batch;
@@ -945,17 +969,28 @@ int segment_states(const char* fn, const WalkArgs& a, int roles, hipStream_t str
   return check_launch(fn);
 }
 
-WalkArgs common_args(const Shape& s, const int32_t* cu, const float* log_decay, int terms) {
+WalkArgs common_args(const Shape& s, const int32_t* cu, const float* log_decay, float scale, int terms) {
   WalkArgs a = {};
   a.cu = cu;
   a.log_decay = log_decay;
+  a.scale = scale;
   a.total = s.total;
   a.batch = s.batch;
   a.kv_heads = s.kv_heads;
-  a.seg = segment_tokens(s.total, s.heads);
+  a.seg = segment_tokens(s.total, s.kv_heads);
   a.slots = (int)slot_count(s.total, s.batch, a.seg);
   a.terms = terms;
   return a;
+}
+
+// Query heads that a workgroup walks together: as many of a group as leave the
+// GPU kLinWalks workgroups.  They share the update of the state, its load and
+// the rows of k and v.
+constexpr int64_t kLinWalks = 512;
+int heads_together(const WalkArgs& a, int group) {
+  int n = group;
+  while (n > 1 && (group % n || (int64_t)a.slots * a.kv_heads * (group / n) < kLinWalks)) --n;
+  return n;
 }
 
 // 16-bit operands of a weighted row in the states' updates: 16 (bf16) or 22
@@ -967,47 +1002,59 @@ template <typename T>
 int run_fwd(const char* fn, const Shape& s, const void* q, const void* k, const void* v, void* o,
             const float* log_decay, const int32_t* cu, const float* init, float* last,
             const int64_t* st, float scale, void* workspace, hipStream_t stream) {
-  WalkArgs a = common_args(s, cu, log_decay, update_terms(s.dtype, last != nullptr));
+  WalkArgs a = common_args(s, cu, log_decay, scale, update_terms(s.dtype, last != nullptr));
   const int group = s.heads / s.kv_heads;
   a.role[0] = {q, k, v, o, st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7],
                init, last, static_cast<float*>(workspace), s.dv, 1,
-               s.heads, group, 1, s.dk, s.dv, 0, 0, scale, scale, 1.f};
+               group, heads_together(a, group), 1, s.dk, s.dv, 0, 0, 1.f, 1.f};
   if (s.total > a.seg)
     if (int rc = segment_states<T>(fn, a, 1, stream)) return rc;
-  return walk<T, true>(fn, a, 1, stream);
+  return walk_out<T>(fn, a, 1, stream);
 }
 
+// The carried state of the backward is R / scale (its operands are then the
+// rows themselves): the final state's gradient comes in divided by scale, the
+// initial state's goes out multiplied.
 template <typename T>
 int run_bwd(const char* fn, const Shape& s, const void* dout, const void* q, const void* k, const void* v,
             void* dq, void* dk, void* dv, const float* log_decay, const int32_t* cu, const float* init,
-            const float* dlast, float* dinit, const int64_t* st, float scale, void* workspace,
-            hipStream_t stream) {
-  WalkArgs a = common_args(s, cu, log_decay, update_terms(s.dtype, dinit != nullptr));
+            const float* dlast, float* dinit, const float* fwd_states, const int64_t* st, float scale,
+            void* workspace, hipStream_t stream) {
+  WalkArgs a = common_args(s, cu, log_decay, scale, update_terms(s.dtype, dinit != nullptr));
   const int group = s.heads / s.kv_heads;
-  float* seg_s = static_cast<float*>(workspace);
-  float* seg_r = seg_s + states_bytes(s) / sizeof(float);
   const int64_t *sdo = st, *sq = st + 2, *sk = st + 4, *sv = st + 6, *sdq = st + 8, *sdk = st + 10, *sdv = st + 12;
+  float* seg_r = static_cast<float*>(workspace);
+  // only written when the forward's are not at hand
+  float* seg_s = fwd_states ? const_cast<float*>(fwd_states) : seg_r + states_bytes(s) / sizeof(float);
+  const float inv = 1.f / scale;
   if (s.total > a.seg) {
-    // S forward from (k, v), R backward from (q, dout), both dk x dv
-    a.role[0] = {nullptr, k, v, nullptr, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0,
-                 init, nullptr, seg_s, s.dv, 1, s.heads, group, 1, s.dk, s.dv, 0, 0, 1.f, 1.f, 1.f};
-    a.role[1] = {nullptr, q, dout, nullptr, 0, 0, sq[0], sq[1], sdo[0], sdo[1], 0, 0,
-                 dlast, nullptr, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 0, 1.f, 1.f, scale};
-    if (int rc = segment_states<T>(fn, a, 2, stream)) return rc;
+    // R backward from (q, dout), S forward from (k, v), both dk x dv
+    a.role[0] = {nullptr, q, dout, nullptr, 0, 0, sq[0], sq[1], sdo[0], sdo[1], 0, 0,
+                 dlast, nullptr, seg_r, s.dv, 1, 1, 1, group, s.dk, s.dv, 1, 0, inv, 1.f};
+    a.role[1] = {nullptr, k, v, nullptr, 0, 0, sk[0], sk[1], sv[0], sv[1], 0, 0,
+                 init, nullptr, seg_s, s.dv, 1, 1, 1, 1, s.dk, s.dv, 0, 0, 1.f, 1.f};
+    if (int rc = segment_states<T>(fn, a, fwd_states ? 1 : 2, stream)) return rc;
   }
   const Role rdq = {dout, v, k, dq, sdo[0], sdo[1], sv[0], sv[1], sk[0], sk[1], sdq[0], sdq[1],
-                    init, nullptr, seg_s, 1, s.dv, s.heads, group, 1, s.dv, s.dk, 0, 1, scale, scale, 1.f};
+                    init, nullptr, seg_s, 1, s.dv, group, heads_together(a, group), 1, s.dv, s.dk, 0, 1, 1.f, 1.f};
   const Role rdk = {v, dout, q, dk, sv[0], sv[1], sdo[0], sdo[1], sq[0], sq[1], sdk[0], sdk[1],
-                    dlast, nullptr, seg_r, 1, s.dv, s.kv_heads, 1, group, s.dv, s.dk, 1, 1, scale, 1.f, scale};
+                    dlast, nullptr, seg_r, 1, s.dv, 1, 1, group, s.dv, s.dk, 1, 1, inv, 1.f};
   const Role rdv = {k, q, dout, dv, sk[0], sk[1], sq[0], sq[1], sdo[0], sdo[1], sdv[0], sdv[1],
-                    dlast, dinit, seg_r, s.dv, 1, s.kv_heads, 1, group, s.dk, s.dv, 1, 1, scale, 1.f, scale};
+                    dlast, dinit, seg_r, s.dv, 1, 1, 1, group, s.dk, s.dv, 1, 1, inv, scale};
+  // dk first and dv beside it: they read the same rows in the same order
   a.role[0] = rdk;
-  a.role[1] = rdq;
-  a.role[2] = rdv;
-  if (s.dk == s.dv) return walk<T, true>(fn, a, 3, stream);
-  if (int rc = walk<T, true>(fn, a, 2, stream)) return rc;
-  a.role[0] = rdv;
-  return walk<T, true>(fn, a, 1, stream);
+  if (s.dk == s.dv) {
+    a.role[1] = rdv;
+    a.role[2] = rdq;
+    if (rdq.x_loop == 1) return walk_out<T>(fn, a, 3, stream);
+    if (int rc = walk_out<T>(fn, a, 2, stream)) return rc;
+  } else {
+    if (int rc = walk_out<T>(fn, a, 1, stream)) return rc;
+    a.role[0] = rdv;
+    if (int rc = walk_out<T>(fn, a, 1, stream)) return rc;
+  }
+  a.role[0] = rdq;
+  return walk_out<T>(fn, a, 1, stream);
 }
 
 template <typename T>
@@ -1074,8 +1121,8 @@ extern "C" int scree_linear_attn_fwd(const void* q, const void* k, const void* v
 extern "C" int scree_linear_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
                                      const float* log_decay, void* dq, void* dk, void* dv,
                                      const float* initial_state, const float* dfinal_state,
-                                     float* dinitial_state, const int32_t* cu_seqlens, int batch,
-                                     int64_t total_tokens, int heads, int kv_heads, int k_dim,
+                                     float* dinitial_state, const void* fwd_workspace,
+                                     const int32_t* cu_seqlens, int batch, int64_t total_tokens, int heads, int kv_heads, int k_dim,
                                      int v_dim, const int64_t* strides, float scale, int dtype,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "scree_linear_attn_bwd";
@@ -1083,8 +1130,10 @@ extern "C" int scree_linear_attn_bwd(const void* dout, const void* q, const void
   if (int rc = check_shape(fn, s)) return rc;
   if (!cu_seqlens || !log_decay || !strides)
     return set_error(SCREE_ERR_INVALID, "%s: cu_seqlens, log_decay or strides is null", fn);
-  const void* states[] = {initial_state, dfinal_state, dinitial_state};
-  if (int rc = check_states(fn, states, 3)) return rc;
+  const void* states[] = {initial_state, dfinal_state, dinitial_state, fwd_workspace};
+  if (int rc = check_states(fn, states, 4)) return rc;
+  if (scale == 0.f || !(scale - scale == 0.f))
+    return set_error(SCREE_ERR_INVALID, "%s: scale must be finite and not zero", fn);
   if (total_tokens) {
     const Arg args[] = {{"dout", dout, strides, v_dim}, {"q", q, strides + 2, k_dim},
                         {"k", k, strides + 4, k_dim}, {"v", v, strides + 6, v_dim},
@@ -1094,18 +1143,18 @@ extern "C" int scree_linear_attn_bwd(const void* dout, const void* q, const void
   } else if (!dinitial_state) {
     return SCREE_OK;
   }
-  const size_t need = 2 * states_bytes(s);
+  const size_t need = (fwd_workspace ? 1 : 2) * states_bytes(s);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return set_error(SCREE_ERR_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", fn, need,
                      workspace ? workspace_bytes : (size_t)0);
   hipStream_t hs = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case SCREE_DTYPE_F32:
-      return run_bwd<float>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, strides, scale, workspace, hs);
+      return run_bwd<float>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, static_cast<const float*>(fwd_workspace), strides, scale, workspace, hs);
     case SCREE_DTYPE_F16:
-      return run_bwd<f16>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, strides, scale, workspace, hs);
+      return run_bwd<f16>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, static_cast<const float*>(fwd_workspace), strides, scale, workspace, hs);
     default:
-      return run_bwd<bf16>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, strides, scale, workspace, hs);
+      return run_bwd<bf16>(fn, s, dout, q, k, v, dq, dk, dv, log_decay, cu_seqlens, initial_state, dfinal_state, dinitial_state, static_cast<const float*>(fwd_workspace), strides, scale, workspace, hs);
   }
 }
 

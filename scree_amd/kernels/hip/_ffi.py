@@ -67,7 +67,7 @@ _SIGNATURES = {
     "scree_linear_attn_workspace_bytes": (_S, [_I, _L, _I, _I, _I, _I, _I]),
     "scree_linear_attn_fwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _I, _I, _I, _I, _P, _F, _I,
                                    _P, _S, _P]),
-    "scree_linear_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _I, _I, _I,
+    "scree_linear_attn_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _I, _I, _I,
                                    _I, _P, _F, _I, _P, _S, _P]),
     "scree_linear_attn_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _F, _I, _P]),
     "scree_token_logprobs_workspace_bytes": (_S, [_L, _L, _I]),

@@ -88,6 +88,8 @@ def _strides(ts):
 
 
 def linear_fwd(q, k, v, log_decay, cu, scale, init, want_state, out):
+    """``(final states or None, workspace or None)``; the backward of the same
+    call can take the workspace's states."""
     batch = cu.numel() - 1
     last = None
     if want_state:
@@ -98,22 +100,22 @@ def linear_fwd(q, k, v, log_decay, cu, scale, init, want_state, out):
                 log_decay.data_ptr(), out.data_ptr(), _ffi.ptr(init), _ffi.ptr(last), cu.data_ptr(),
                 batch, q.shape[0], q.shape[1], k.shape[1], q.shape[2], v.shape[2],
                 _strides((q, k, v, out)), scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
-    return last
+    return last, ws
 
 
-def linear_bwd(do, q, k, v, log_decay, cu, scale, init, dlast, want_dinit):
+def linear_bwd(do, q, k, v, log_decay, cu, scale, init, dlast, want_dinit, fwd_ws=None):
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     batch = cu.numel() - 1
     dinit = None
     if want_dinit:
         dinit = torch.empty((batch, k.shape[1], k.shape[2], v.shape[2]), dtype=torch.float32,
                             device=q.device)
-    ws, nws = _workspace(cu, q, k, v, True)
+    ws, nws = _workspace(cu, q, k, v, fwd_ws is None)
     _ffi.launch(_ffi.lib().scree_linear_attn_bwd, q, do.data_ptr(), q.data_ptr(), k.data_ptr(),
                 v.data_ptr(), log_decay.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                _ffi.ptr(init), _ffi.ptr(dlast), _ffi.ptr(dinit), cu.data_ptr(), batch, q.shape[0],
-                q.shape[1], k.shape[1], q.shape[2], v.shape[2], _strides((do, q, k, v, dq, dk, dv)),
-                scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
+                _ffi.ptr(init), _ffi.ptr(dlast), _ffi.ptr(dinit), _ffi.ptr(fwd_ws), cu.data_ptr(), batch,
+                q.shape[0], q.shape[1], k.shape[1], q.shape[2], v.shape[2],
+                _strides((do, q, k, v, dq, dk, dv)), scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
     return dq, dk, dv, dinit
 
 
@@ -122,21 +124,22 @@ class _LinearAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, log_decay, cu, scale, init, want_state):
         qk, kk, vk, s0 = _view(q), _view(k), _view(v), _state(init)
         out = torch.empty((*q.shape[:2], v.shape[2]), dtype=q.dtype, device=q.device)
-        last = linear_fwd(qk, kk, vk, log_decay, cu, scale, s0, want_state, out)
-        ctx.save_for_backward(qk, kk, vk, log_decay, cu, s0)
+        # the workspace's states between segments serve the backward too
+        last, ws = linear_fwd(qk, kk, vk, log_decay, cu, scale, s0, want_state, out)
+        ctx.save_for_backward(qk, kk, vk, log_decay, cu, s0, ws)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return (out, last) if want_state else out
 
     @staticmethod
     def backward(ctx, do, dlast=None):
-        q, k, v, log_decay, cu, s0 = ctx.saved_tensors
+        q, k, v, log_decay, cu, s0, ws = ctx.saved_tensors
         if do is None and dlast is None:
             return (None,) * 8
         if do is None:
             do = torch.zeros((*q.shape[:2], v.shape[2]), dtype=q.dtype, device=q.device)
         dq, dk, dv, dinit = linear_bwd(_view(do), q, k, v, log_decay, cu, ctx.scale, s0,
-                                       _state(dlast), ctx.needs_input_grad[6])
+                                       _state(dlast), ctx.needs_input_grad[6], ws)
         return dq, dk, dv, None, None, None, dinit, None
 
 
@@ -180,8 +183,8 @@ def varlen_linear_attention_hip(q, k, v, log_decay, cu_seqlens, scale=None, init
         assert out.shape == shape and out.dtype == q.dtype and out.device == q.device, (
             "out must be (total_tokens, heads, v_dim) like q")
     ok = _view(out)
-    last = linear_fwd(_view(q), _view(k), _view(v), log_decay.contiguous(), cu, scale,
-                      _state(initial_state), return_state, ok)
+    last, _ = linear_fwd(_view(q), _view(k), _view(v), log_decay.contiguous(), cu, scale,
+                         _state(initial_state), return_state, ok)
     if ok is not out:
         out.copy_(ok)
     return (out, last) if return_state else out

@@ -127,9 +127,18 @@ def test_c_abi_refusals():
     need = lib.scree_linear_attn_workspace_bytes(2, 100000, 4, 4, 64, 64, 0)
     assert need > 0 and lib.scree_linear_attn_workspace_bytes(2, 100000, 4, 4, 64, 64, 1) == 2 * need
     assert lib.scree_linear_attn_workspace_bytes(2, 200, 4, 4, 64, 64, 1) == 0
-    rc = lib.scree_linear_attn_bwd(p, p, p, p, p, p, p, null, null, null, null, p, 2, 10, 4, 4, 64, 64, st,
-                                   1.0, 1, null, 0, null)
-    assert rc == _ffi.SCREE_ERR_INVALID and "dv is null" in err()
+
+    def bwd(dv=p, fwd=null, n=10, scale=1.0, ws=null, nws=0):
+        return lib.scree_linear_attn_bwd(p, p, p, p, p, p, p, dv, null, null, null, fwd, p, 2, n, 4, 4, 64, 64,
+                                         st, scale, 1, ws, nws, null)
+
+    assert bwd(dv=null) == _ffi.SCREE_ERR_INVALID and "dv is null" in err()
+    assert bwd(fwd=odd) == _ffi.SCREE_ERR_INVALID and "aligned" in err()
+    for scale in (0.0, float("nan"), float("inf")):
+        assert bwd(scale=scale) == _ffi.SCREE_ERR_INVALID and "scale" in err()
+    # the forward's states at hand, half the room is enough
+    assert bwd(n=100000, ws=p, nws=2 * need - 1) == _ffi.SCREE_ERR_WORKSPACE
+    assert bwd(n=100000, ws=p, nws=need - 1, fwd=p) == _ffi.SCREE_ERR_WORKSPACE
     rows = _ffi.int64_array([256, 64] * 4 + [4 * 64 * 64, 4 * 64 * 64 - 4])
     rc = lib.scree_linear_attn_step(p, p, p, p, p, p, p, 2, 4, 4, 64, 64, rows, 1.0, 1, null)
     assert rc == _ffi.SCREE_ERR_INVALID and "state row stride" in err()
