@@ -835,14 +835,23 @@ __global__ __launch_bounds__(kStepThreads) void lin_step_kernel(StepArgs a) {
 // ------------------------------------------------------------------- host
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Tokens per segment: enough segments to give the GPU kLinFill workgroups, of
-// at least kLinMinSeg tokens (their states cost as much traffic as that many
-// tokens) and at most kLinMaxSeg (the longest walk).
-constexpr int64_t kLinFill = 1024;
-constexpr int kLinMinSeg = 256, kLinMaxSeg = 2048;
+// Tokens per segment.  The walks' workgroups, a segment and K/V head each, are
+// best one round of kLinFill (two for each CU; a sequence has half a segment
+// more than its tokens fill, on average): 65,536 tokens x 16 heads of 128 take
+// 412 us in segments of 2,048, 463 in 1,024 and 527 in 512, and the fewer
+// segments the less traffic of their states (64 KB each, read and written five
+// times).  At least kLinMinSeg, at most kLinMaxSeg, so that one long sequence
+// among many heads does not outlast the rest (config 5: 2,667 us at 4,096,
+// 2,818 at 2,048).  A small batch of short sequences is one segment each: two
+// launches less (22 us against 29 at 1,980 tokens of 16 sequences).
+constexpr int64_t kLinFill = 512;
+constexpr int kLinMinSeg = 128, kLinMaxSeg = 4096;
+constexpr int kLinSmall = 2048, kLinSmallMean = 256;
 
-inline int segment_tokens(int64_t total, int kv_heads) {
-  int64_t m = (total * kv_heads / kLinFill + 63) / 64 * 64;
+inline int segment_tokens(int64_t total, int batch, int kv_heads) {
+  if (total <= kLinSmall && total <= (int64_t)batch * kLinSmallMean && batch >= 8) return kLinSmall;
+  const int64_t room = kLinFill / kv_heads - batch / 2;
+  int64_t m = room < 1 ? kLinMaxSeg : ((total + room - 1) / room + 63) / 64 * 64;
   if (m < kLinMinSeg) m = kLinMinSeg;
   if (m > kLinMaxSeg) m = kLinMaxSeg;
   return (int)m;
@@ -898,7 +907,7 @@ int check_states(const char* fn, const void* const* p, int n) {
 
 // Bytes of one set of segment states (0: no sequence can have two segments).
 size_t states_bytes(const Shape& s) {
-  const int seg = segment_tokens(s.total, s.kv_heads);
+  const int seg = segment_tokens(s.total, s.batch, s.kv_heads);
   if (s.total <= seg) return 0;
   return (size_t)slot_count(s.total, s.batch, seg) * s.kv_heads * s.dk * s.dv * sizeof(float);
 }
@@ -977,7 +986,7 @@ WalkArgs common_args(const Shape& s, const int32_t* cu, const float* log_decay, 
   a.total = s.total;
   a.batch = s.batch;
   a.kv_heads = s.kv_heads;
-  a.seg = segment_tokens(s.total, s.kv_heads);
+  a.seg = segment_tokens(s.total, s.batch, s.kv_heads);
   a.slots = (int)slot_count(s.total, s.batch, a.seg);
   a.terms = terms;
   return a;
@@ -986,7 +995,7 @@ WalkArgs common_args(const Shape& s, const int32_t* cu, const float* log_decay, 
 // Query heads that a workgroup walks together: as many of a group as leave the
 // GPU kLinWalks workgroups.  They share the update of the state, its load and
 // the rows of k and v.
-constexpr int64_t kLinWalks = 512;
+constexpr int64_t kLinWalks = 256;
 int heads_together(const WalkArgs& a, int group) {
   int n = group;
   while (n > 1 && (group % n || (int64_t)a.slots * a.kv_heads * (group / n) < kLinWalks)) --n;

@@ -151,9 +151,9 @@ def test_grouped_heads(dtype, h, hk, state):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("lengths", [[1500], [700, 0, 1, 300, 256, 257, 1100], [255, 256, 257, 512, 513]])
+@pytest.mark.parametrize("lengths", [[1500], [700, 0, 1, 300, 256, 257, 1100], [127, 128, 129, 512, 513]])
 def test_segmented_sequences(dtype, lengths):
-    """Past 256 tokens a sequence is walked in several segments."""
+    """Long sequences are walked in several segments (here of 128 tokens)."""
     from scree_amd.kernels.hip.linear_attention import workspace_bytes
 
     assert workspace_bytes(len(lengths), sum(lengths), 2, 1, 64, 64, False) > 0

@@ -126,7 +126,9 @@ def test_c_abi_refusals():
         assert fwd(**bad) == code and text in err(), (bad, err())
     need = lib.scree_linear_attn_workspace_bytes(2, 100000, 4, 4, 64, 64, 0)
     assert need > 0 and lib.scree_linear_attn_workspace_bytes(2, 100000, 4, 4, 64, 64, 1) == 2 * need
-    assert lib.scree_linear_attn_workspace_bytes(2, 200, 4, 4, 64, 64, 1) == 0
+    assert lib.scree_linear_attn_workspace_bytes(2, 100, 4, 4, 64, 64, 1) == 0
+    # a small batch of short sequences is walked whole
+    assert lib.scree_linear_attn_workspace_bytes(16, 1980, 4, 4, 32, 32, 1) == 0
 
     def bwd(dv=p, fwd=null, n=10, scale=1.0, ws=null, nws=0):
         return lib.scree_linear_attn_bwd(p, p, p, p, p, p, p, dv, null, null, null, fwd, p, 2, n, 4, 4, 64, 64,
