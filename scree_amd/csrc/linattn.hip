@@ -515,6 +515,23 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
           for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+          // a state past fp16's range goes in scaled by a power of two
+          float down = 1.f, up = 1.f;
+          if constexpr (__is_same(T, f16)) {
+            float top = 0.f;
+#pragma unroll
+            for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+              for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(st[m][u][i]));
+            if (__ballot(top > 32768.f)) {
+#pragma unroll
+              for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+              up = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top) - 15);
+              down = 1.f / up;
+            }
+          }
 #pragma unroll
           for (int k = 0; k < DX / 32; ++k) {
             // reads hoisted over several k would not fit the registers
@@ -530,6 +547,10 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
                 f[i] = st[2 * k][u][i];
                 f[4 + i] = st[2 * k + 1][u][i];
               }
+              if constexpr (__is_same(T, f16))
+                if (down != 1.f)
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) f[i] *= down;
               if constexpr (sizeof(T) == 2) {
                 const F hi = take<T>(f);
 #pragma unroll
@@ -542,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
           }
 #pragma unroll
           for (int s = 0; s < ST; ++s) {
-            const float w = wi[16 * s];
+            const float w = wi[16 * s] * up;
 #pragma unroll
             for (int u = 0; u < NT; ++u) o[u][s] *= w;
           }

@@ -25,42 +25,65 @@ import math
 import torch
 
 from . import _ffi
-from .attention import _cu, _kernel_view
+from .attention import _MAX_STRIDE, _cu
 
 MAX_DIM = 256
 
 
-def _check(q, k, v, log_decay):
-    assert q.is_cuda, "linear attention on HIP requires ROCm device tensors"
-    assert q.dim() == k.dim() == v.dim() == 3, "q, k, v must be (tokens, heads, head_dim)"
-    assert k.shape[:2] == v.shape[:2], "k and v must share tokens and heads"
-    assert q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2], (
-        "q and k must share tokens and head_dim")
-    assert k.shape[1] >= 1 and q.shape[1] >= 1 and q.shape[1] % k.shape[1] == 0, (
+@functools.lru_cache(maxsize=256)
+def _shape_plan(qs, ks, vs, dtype):
+    """Checks that depend on shapes and dtype alone; ``(dtype code, default scale)``."""
+    assert len(qs) == len(ks) == len(vs) == 3, "q, k, v must be (tokens, heads, head_dim)"
+    assert ks[:2] == vs[:2], "k and v must share tokens and heads"
+    assert qs[0] == ks[0] and qs[2] == ks[2], "q and k must share tokens and head_dim"
+    assert ks[1] >= 1 and qs[1] >= 1 and qs[1] % ks[1] == 0, (
         "k/v heads must divide q heads (grouped-query attention)")
-    for d in (q.shape[2], v.shape[2]):
+    for d in (qs[2], vs[2]):
         assert 8 <= d <= MAX_DIM and d % 8 == 0, "head dims must be multiples of 8 up to 256"
-    assert q.dtype in (torch.float16, torch.bfloat16, torch.float32), f"unsupported dtype {q.dtype}"
+    assert dtype in (torch.float16, torch.bfloat16, torch.float32), f"unsupported dtype {dtype}"
+    return _ffi.dtype_code(dtype), 1.0 / math.sqrt(qs[2])
+
+
+def _check(q, k, v, log_decay):
+    dev = q.get_device()
+    assert dev >= 0, "linear attention on HIP requires ROCm device tensors"
+    plan = _shape_plan(q.shape, k.shape, v.shape, q.dtype)
     assert q.dtype == k.dtype == v.dtype, "q, k, v must share a dtype"
-    assert q.device == k.device == v.device, "q, k, v must be on the same device"
+    assert dev == k.get_device() == v.get_device(), "q, k, v must be on the same device"
     assert log_decay.shape == k.shape[1:2] and log_decay.dtype == torch.float32, (
         "log_decay must be float32, one per K/V head")
-    assert log_decay.device == q.device, "log_decay must be on q's device"
-    if torch.is_grad_enabled() and log_decay.requires_grad:
+    assert log_decay.get_device() == dev, "log_decay must be on q's device"
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("log_decay is a constant of the head: it has no gradient here")
+    return plan
 
 
 def _check_state(s, name, batch, k, v):
-    assert s.shape == (batch, k.shape[1], k.shape[2], v.shape[2]), (
+    assert s.shape == (batch, *k.shape[1:], v.shape[2]), (
         f"{name} must be (batch, kv_heads, k_dim, v_dim)")
     assert s.dtype == torch.float32, f"{name} must be float32"
-    assert s.device == k.device, f"{name} must be on q's device"
+    assert s.get_device() == k.get_device(), f"{name} must be on q's device"
+
+
+def _row_head(t):
+    """Row and head strides; those of an axis of one are the contiguous ones."""
+    n, h, d = t.shape
+    s0, s1, _ = t.stride()
+    if h == 1:
+        s1 = d
+    return (h * d if n <= 1 else s0), s1
 
 
 def _view(t):
     """``t`` itself when the library can read it in place, else an aligned copy."""
-    t = _kernel_view(t)
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        s0, s1 = _row_head(t)
+        if (t.stride(2) == 1 and s0 % 8 == 0 and s1 % 8 == 0 and 0 <= s1 < _MAX_STRIDE
+                and t.shape[2] <= s0 < _MAX_STRIDE):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _state(s):
@@ -83,8 +106,8 @@ def _workspace(cu, q, k, v, backward):
     return (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None), n
 
 
-def _strides(ts):
-    return _ffi.int64_array(sum((t.stride()[:2] for t in ts), ()))
+def _strides(ts, extra=()):
+    return _ffi.int64_array(sum([_row_head(t) for t in ts], ()) + extra)
 
 
 def linear_fwd(q, k, v, log_decay, cu, scale, init, want_state, out):
@@ -144,12 +167,12 @@ class _LinearAttentionFn(torch.autograd.Function):
 
 
 def _prepare(q, k, v, log_decay, cu_seqlens, scale, initial_state):
-    _check(q, k, v, log_decay)
+    _, default_scale = _check(q, k, v, log_decay)
     cu = _cu(cu_seqlens, q.device)
     assert cu.dim() == 1 and cu.numel() >= 2, "cu_seqlens must have batch + 1 entries"
     if initial_state is not None:
         _check_state(initial_state, "initial_state", cu.numel() - 1, k, v)
-    return cu, 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    return cu, default_scale if scale is None else float(scale)
 
 
 def varlen_linear_attention_hip(q, k, v, log_decay, cu_seqlens, scale=None, initial_state=None,
@@ -207,10 +230,16 @@ def varlen_linear_attention_hip_backward(do, q, k, v, log_decay, cu_seqlens, sca
                       _state(initial_state), _state(dstate), initial_state is not None)
 
 
-def _step_rows(s, name):
-    assert s.stride()[1:] == (s.shape[2] * s.shape[3], s.shape[3], 1) and s.stride(0) % 4 == 0 and (
-        s.shape[0] <= 1 or s.stride(0) >= s[0].numel()) and s.data_ptr() % 16 == 0, (
+def _step_state(s, name, batch, k, v):
+    _check_state(s, name, batch, k, v)
+    _, hk, dk, dv = s.shape
+    s0, s1, s2, s3 = s.stride()
+    if batch <= 1:
+        s0 = hk * dk * dv
+    assert (s1 == dk * dv or hk == 1) and s2 == dv and s3 == 1 and s0 % 4 == 0 and (
+        s0 >= hk * dk * dv) and s.data_ptr() % 16 == 0, (
         f"{name} must hold each row's state contiguously, 16-byte aligned")
+    return s0
 
 
 def linear_attention_step_hip(q, k, v, log_decay, state, scale=None, state_out=None, out=None):
@@ -224,33 +253,29 @@ def linear_attention_step_hip(q, k, v, log_decay, state, scale=None, state_out=N
     ``(batch, heads, v_dim)``; one step of what
     :func:`varlen_linear_attention_hip` computes.  No gradient is recorded.
     """
-    _check(q, k, v, log_decay)
-    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))), (
+    code, default_scale = _check(q, k, v, log_decay)
+    assert not ((q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)
+                and torch.is_grad_enabled()), (
         "a decoding step records no gradient; use varlen_linear_attention_hip")
-    b = q.shape[0]
-    _check_state(state, "state", b, k, v)
-    _step_rows(state, "state")
+    b, h, dk = q.shape
+    hk, dv = v.shape[1:]
+    rows = _step_state(state, "state", b, k, v)
     if state_out is None:
-        state_out = state
+        state_out, rows_out = state, rows
     else:
-        _check_state(state_out, "state_out", b, k, v)
-        _step_rows(state_out, "state_out")
-    shape = (*q.shape[:2], v.shape[2])
+        rows_out = _step_state(state_out, "state_out", b, k, v)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty((b, h, dv), dtype=q.dtype, device=q.device)
     else:
-        assert out.shape == shape and out.dtype == q.dtype and out.device == q.device, (
+        assert out.shape == (b, h, dv) and out.dtype == q.dtype and out.device == q.device, (
             "out must be (batch, heads, v_dim) like q")
     if b == 0:
         return out
     qk, kk, vk, ok = _view(q), _view(k), _view(v), _view(out)
-    strides = _ffi.int64_array(qk.stride()[:2] + kk.stride()[:2] + vk.stride()[:2] + ok.stride()[:2]
-                               + (state.stride(0), state_out.stride(0)))
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     _ffi.launch(_ffi.lib().scree_linear_attn_step, qk, qk.data_ptr(), kk.data_ptr(), vk.data_ptr(),
                 log_decay.contiguous().data_ptr(), ok.data_ptr(), state.data_ptr(),
-                state_out.data_ptr(), b, q.shape[1], k.shape[1], q.shape[2], v.shape[2], strides,
-                scale, _ffi.dtype_code(q.dtype))
+                state_out.data_ptr(), b, h, hk, dk, dv, _strides((qk, kk, vk, ok), (rows, rows_out)),
+                default_scale if scale is None else float(scale), code)
     if ok is not out:
         out.copy_(ok)
     return out

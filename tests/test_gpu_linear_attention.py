@@ -176,6 +176,18 @@ def test_strong_decays_and_none(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_states_past_the_range_of_fp16(dtype):
+    """Sums of k v^T of 1e6 and more under small queries: outputs of ordinary size."""
+    for h, hk in ((2, 2), (4, 1)):
+        t = _inputs([400, 900], h, hk, 64, 64, dtype, 5, True, True)
+        t["k"], t["v"] = t["k"] * 20, (t["v"] + 2.0) * 30
+        t["q"], t["do"] = t["q"] * 1e-3, t["do"] * 1e-3
+        t["g"] = torch.zeros(hk).cuda()
+        o, last = _check([400, 900], h, hk, 64, 64, dtype, t=t)
+        assert last.abs().max() > 1e5 and torch.isfinite(o).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_strided_views_and_unaligned_inputs(dtype):
     from scree_amd.kernels.hip import varlen_linear_attention_hip
 
