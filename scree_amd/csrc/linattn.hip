@@ -227,8 +227,8 @@ __device__ __forceinline__ typename Frag<T>::t take(float (&rest)[8]) {
     } else {
       const auto h = __builtin_amdgcn_cvt_pkrtz(rest[j], rest[j + 1]);
       w[j / 2] = __builtin_bit_cast(uint32_t, h);
-      rest[j] -= (float)h[0];
-      rest[j + 1] -= (float)h[1];
+      rest[j] = fmaf((float)h[0], -1.f, rest[j]);  // v_fma_mix_f32
+      rest[j + 1] = fmaf((float)h[1], -1.f, rest[j + 1]);
     }
   }
   return __builtin_bit_cast(typename Frag<T>::t, make_uint4(w[0], w[1], w[2], w[3]));
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   const float *wp = pow_s + c - 4 * g, *wi = pow_s + c + e;
   const float* wz0 = pow - e - LX::TOK_G * g;
   // operands of a weighted row: an output state gets as many as fp32 has bits for
-  const bool three = sizeof(T) == 2 && a.terms > 2 && (!OUT || sg.index == final);
+  const bool three = __is_same(T, bf16) && a.terms > 2 && (!OUT || sg.index == final);
 
   f32x4 o[NT][OUT ? ST : 1];
   for (int ci = 0; ci < chunks; ++ci) {
@@ -555,12 +555,8 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
         // out^T = (X A)^T lam^{i+e}: the state's accumulators are its operand as
         // they lie, in two 16-bit operands
         if (over_x || turn == 0) {
-#pragma unroll
-          for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int s = 0; s < ST; ++s) o[u][s] = f32x4{0.f, 0.f, 0.f, 0.f};
           // a state past fp16's range goes in scaled by a power of two
-          float down = 1.f, up = 1.f;
+          float up = 1.f;
           if constexpr (__is_same(T, f16)) {
             float top = 0.f;
 #pragma unroll
@@ -572,8 +568,13 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
             if (__ballot(top > 32768.f)) {
 #pragma unroll
               for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-              up = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top) - 15);
-              down = 1.f / up;
+              const int over = __builtin_amdgcn_frexp_expf(top) - 15;
+              up = __builtin_amdgcn_ldexpf(1.f, over);
+              const float down = __builtin_amdgcn_ldexpf(1.f, -over);
+#pragma unroll
+              for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) st[m][u] *= down;
             }
           }
 #pragma unroll
@@ -585,24 +586,27 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
             for (int s = 0; s < ST; ++s) xf[s] = LX::row44(x44, 16 * s, 32 * k);
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
+              const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
               float f[8];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 f[i] = st[2 * k][u][i];
                 f[4 + i] = st[2 * k + 1][u][i];
               }
-              if constexpr (__is_same(T, f16))
-                if (down != 1.f)
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) f[i] *= down;
               if constexpr (sizeof(T) == 2) {
                 const F hi = take<T>(f);
 #pragma unroll
-                for (int s = 0; s < ST; ++s) mma(o[u][s], hi, xf[s]);
+                for (int s = 0; s < ST; ++s) {
+                  if (k == 0) o[u][s] = zero;
+                  mma(o[u][s], hi, xf[s]);
+                }
               }
               const F lo = to_frag<T>(f);
 #pragma unroll
-              for (int s = 0; s < ST; ++s) mma(o[u][s], lo, xf[s]);
+              for (int s = 0; s < ST; ++s) {
+                if (sizeof(T) == 4 && k == 0) o[u][s] = zero;
+                mma(o[u][s], lo, xf[s]);
+              }
             }
           }
 #pragma unroll
@@ -611,6 +615,12 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
 #pragma unroll
             for (int u = 0; u < NT; ++u) o[u][s] *= w;
           }
+          if constexpr (__is_same(T, f16))
+            if (up != 1.f)
+#pragma unroll
+              for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) st[m][u] *= up;
         }
         __syncthreads();
       }
@@ -680,15 +690,18 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
         if (!over_x && !last_turn) continue;
         const int64_t low = chunk_low(ci, n);
         T* out = static_cast<T*>(r.out) + (sg.row0 + low) * r.o_row + (head + (over_x ? turn : 0)) * r.o_head + z0 + CW * wave;
-        // row i of the chunk lies at i, or at n - 1 - i
+        // row i of the chunk lies at i, or at n - 1 - i: this lane's row of a strip,
+        // and the step to the next strip's
+        const int row = (NT == 1 && sizeof(T) == 2 ? 16 * (g & 1) : 0) + c;
+        out += (int64_t)(back ? n - 1 - row : row) * r.o_row;
+        const int64_t strip = (back ? -16 : 16) * r.o_row;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
           for (int s = 0; s < ST; ++s) {
-            const int i = 16 * s + c;
-            T* dst = out + (int64_t)(back ? n - 1 - i : i) * r.o_row + 4 * g;
+            T* dst = out + s * strip + 4 * g;
 #pragma unroll
             for (int u = 0; u < NT; ++u)
-              if (i < n && CW * wave + 16 * u + 4 * g < zcols)
+              if (16 * s + row < n && CW * wave + 16 * u + 4 * g < zcols)
                 *reinterpret_cast<float4*>(dst + 16 * u) = make_float4(o[u][s][0], o[u][s][1], o[u][s][2], o[u][s][3]);
           }
         } else if constexpr (NT == 2) {
@@ -700,9 +713,9 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
                                                              false, false);
             const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[1][s][2], o[1][s][3]),
                                                              false, false);
-            const int i = 16 * s + c, col = 16 * (g & 1) + 8 * (g >> 1);
-            if (i < n && CW * wave + col < zcols)
-              st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
+            const int col = 16 * (g & 1) + 8 * (g >> 1);
+            if (16 * s + row < n && CW * wave + col < zcols)
+              st16(out + s * strip + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
           }
         } else {
           // a lane holds 4 columns of a row in every strip; exchanged between two
@@ -713,9 +726,9 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
                                                              false, false);
             const auto e1 = __builtin_amdgcn_permlane16_swap(pack2<T>(o[0][s][2], o[0][s][3]), pack2<T>(o[0][s + 1][2], o[0][s + 1][3]),
                                                              false, false);
-            const int i = 16 * (s + (g & 1)) + c, col = 8 * (g >> 1);
-            if (i < n && CW * wave + col < zcols)
-              st16(out + (int64_t)(back ? n - 1 - i : i) * r.o_row + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
+            const int col = 8 * (g >> 1);
+            if (16 * s + row < n && CW * wave + col < zcols)
+              st16(out + s * strip + col, make_uint4(e0[0], e1[0], e0[1], e1[1]));
           }
         }
       }
