@@ -38,8 +38,12 @@ template <typename T> struct ElemAligned { typedef u32x4_a2 v; };
 template <> struct ElemAligned<float> { typedef u32x4_a4 v; };
 
 // 16 bytes at element alignment: rows of an odd vocabulary start anywhere.
-template <typename T> __device__ __forceinline__ uint4 ld16_elem(const T* p) {
-  const auto v = *reinterpret_cast<const typename ElemAligned<T>::v*>(p);
+// NT: not kept in the caches (kNtBytes).
+template <bool NT, typename T> __device__ __forceinline__ uint4 ld16_elem(const T* p) {
+  const auto* q = reinterpret_cast<const typename ElemAligned<T>::v*>(p);
+  typename ElemAligned<T>::v v;
+  if constexpr (NT) v = __builtin_nontemporal_load(q);
+  else v = *q;
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 template <typename T> __device__ __forceinline__ void st16_elem(T* p, const uint4& u) {
@@ -185,7 +189,7 @@ __device__ __forceinline__ void finish_row(const Stats& a, const TopList& l, con
 
 // Workspace of a split forward: per part 3 floats, then per part top_k
 // (value, index) pairs.
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool NT>
 __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
     const T* __restrict__ logits, int64_t stride, const void* __restrict__ targets, int target_bytes,
     int vocab, int top_k, int parts, int part_cols, float* __restrict__ part_stats,
@@ -213,7 +217,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
     for (int u = 0; u < U; ++u) {
       const int c = base + u * kLpThreads * VEC + lane * VEC;
       have[u] = c < whole;
-      if (have[u]) v[u] = ld16_elem(x + c);
+      if (have[u]) v[u] = ld16_elem<NT>(x + c);
     }
     float mx[U], hi = a.m;
 #pragma unroll
@@ -355,7 +359,7 @@ struct LogprobGrad {
   const float* dtop;
 };
 
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(kLpThreads) void logprob_bwd_kernel(
     const T* __restrict__ logits, int64_t stride, const void* __restrict__ targets, int target_bytes,
     int vocab, int top_k, int parts, int part_cols, LogprobGrad g, T* __restrict__ dlogits,
@@ -404,7 +408,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_bwd_kernel(
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (base + u * kLpThreads * VEC < whole) v[u] = ld16_elem(x + base + u * kLpThreads * VEC);
+      if (base + u * kLpThreads * VEC < whole) v[u] = ld16_elem<NT>(x + base + u * kLpThreads * VEC);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = base + u * kLpThreads * VEC;
@@ -441,6 +445,10 @@ __global__ __launch_bounds__(kLpThreads) void logprob_bwd_kernel(
 constexpr int64_t kLpFill = 1024;
 constexpr int64_t kLpMinCols = 4096;
 constexpr int64_t kLpBwdCols = 16384;
+// Logits that do not fit the 256 MB behind the L2s are gone before the
+// backward reads them: streaming loads take 120 us instead of 135 at 778 MB.
+// At 198 MB they would lose the backward 20 of its 62 us.
+constexpr int64_t kNtBytes = 256ll << 20;
 
 inline int fwd_parts(int64_t rows, int64_t vocab) {
   if (rows >= kLpFill) return 1;
@@ -474,16 +482,15 @@ int launch_fwd(const void* logits, int64_t stride, const void* targets, int targ
                hipStream_t stream) {
   const int parts = fwd_parts(rows, vocab);
   const int cols = part_columns(vocab, parts);
+  const bool nt = rows * vocab * (int64_t)sizeof(T) > kNtBytes;
   float* ps = static_cast<float*>(workspace);
   float2* pt = parts > 1 ? reinterpret_cast<float2*>(ps + (3 * rows * parts + 3) / 4 * 4) : nullptr;
   const dim3 grid((unsigned)(rows * parts));
   const T* x = static_cast<const T*>(logits);
-  if (top_k)
-    hipLaunchKernelGGL((logprob_fwd_kernel<T, true>), grid, dim3(kLpThreads), 0, stream, x, stride,
-                       targets, target_bytes, vocab, top_k, parts, cols, ps, pt, out);
-  else
-    hipLaunchKernelGGL((logprob_fwd_kernel<T, false>), grid, dim3(kLpThreads), 0, stream, x, stride,
-                       targets, target_bytes, vocab, top_k, parts, cols, ps, pt, out);
+  auto kernel = top_k ? (nt ? logprob_fwd_kernel<T, true, true> : logprob_fwd_kernel<T, true, false>)
+                      : (nt ? logprob_fwd_kernel<T, false, true> : logprob_fwd_kernel<T, false, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(kLpThreads), 0, stream, x, stride, targets, target_bytes, vocab,
+                     top_k, parts, cols, ps, pt, out);
   if (parts > 1)
     hipLaunchKernelGGL((logprob_join_kernel<T>), dim3((unsigned)rows), dim3(64), 0, stream, x, stride,
                        targets, target_bytes, vocab, top_k, parts, ps, pt, out);
@@ -495,7 +502,9 @@ int launch_bwd(const void* logits, int64_t stride, const void* targets, int targ
                int64_t rows, int vocab, int top_k, const LogprobGrad& g, void* dlogits,
                int64_t dstride, hipStream_t stream) {
   const int parts = (int)((vocab + kLpBwdCols - 1) / kLpBwdCols);
-  hipLaunchKernelGGL((logprob_bwd_kernel<T>), dim3((unsigned)(rows * parts)), dim3(kLpThreads), 0,
+  const bool nt = rows * vocab * (int64_t)sizeof(T) > kNtBytes;
+  auto kernel = nt ? logprob_bwd_kernel<T, true> : logprob_bwd_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * parts)), dim3(kLpThreads), 0,
                      stream, static_cast<const T*>(logits), stride, targets, target_bytes, vocab,
                      top_k, parts, part_columns(vocab, parts), g, static_cast<T*>(dlogits), dstride);
   return check_launch("scree_token_logprobs_bwd");
