@@ -177,7 +177,9 @@ struct Stage {
   __device__ __forceinline__ void load(const T* base, int64_t row_stride, int n, int d, bool back) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const uint32_t step = (uint32_t)(row_stride * sizeof(T));
-    const __amdgpu_buffer_rsrc_t rs = buffer_of(base, (uint32_t)(n - 1) * step + (uint32_t)(d * sizeof(T)));
+    // 64 rows less than 2^24 elements apart: below 2^32 - 16 bytes
+    const uint32_t bytes = n > 0 ? (uint32_t)(n - 1) * step + (uint32_t)(d * sizeof(T)) : 0u;
+    const __amdgpu_buffer_rsrc_t rs = buffer_of(base, bytes);
     const int r = threadIdx.x / L::CPR, c = threadIdx.x % L::CPR;
     uint32_t at = (uint32_t)(back ? n - 1 - r : r) * step + 16u * c;
     const uint32_t turn = (back ? 0u - RPT : (uint32_t)RPT) * step;

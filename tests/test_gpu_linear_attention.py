@@ -345,12 +345,13 @@ def test_array_level_and_explicit_backward():
         varlen_linear_attention(arrs[0], other, arrs[2], t["g"])
 
 
-def test_graph_replays_match_eager_without_host_sync():
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float32, 128)])  # below and past 64 KB of LDS
+def test_graph_replays_match_eager_without_host_sync(dtype, dim):
     from scree_amd.kernels.hip import varlen_linear_attention_hip_backward, varlen_linear_attention_hip
 
     lengths = [700, 33]
     _, cu = cu_of(lengths)
-    t = _inputs(lengths, 4, 2, 64, 64, torch.bfloat16, 9, True, True)
+    t = _inputs(lengths, 4, 2, dim, dim, dtype, 9, True, True)
 
     def step():
         o, last = varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, initial_state=t["s0"],
@@ -366,10 +367,108 @@ def test_graph_replays_match_eager_without_host_sync():
     with torch.cuda.graph(graph):
         captured = step()
     for seed in range(3):
-        t["q"].copy_(randn(tuple(t["q"].shape), torch.bfloat16, 90 + seed))
+        t["q"].copy_(randn(tuple(t["q"].shape), dtype, 90 + seed))
         want = [x.clone() for x in step()]
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
         for a, b in zip(captured, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_past_2_31_elements(dtype):
+    """Row strides up to the limit of 2^24 elements: places past 2^31."""
+    from scree_amd.kernels.hip import varlen_linear_attention_hip, varlen_linear_attention_hip_backward
+
+    lengths, stride = [3, 127], (1 << 24) - 8
+    _, cu = cu_of(lengths)
+    t = _inputs(lengths, 2, 2, 64, 64, dtype, 5, False, True)
+    far = torch.empty((130 * stride,), dtype=dtype, device="cuda")
+    far_t = {}
+    for i, x in enumerate(("q", "k", "v", "do")):
+        far_t[x] = far.as_strided((130, 2, 64), (stride, 64, 1), 1024 * i)
+        far_t[x].copy_(t[x])
+    out = far.as_strided((130, 2, 64), (stride, 64, 1), 4096)
+    varlen_linear_attention_hip(far_t["q"], far_t["k"], far_t["v"], t["g"], cu, out=out)
+    assert torch.equal(out, varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu))
+    got = varlen_linear_attention_hip_backward(far_t["do"], far_t["q"], far_t["k"], far_t["v"], t["g"], cu)
+    want = varlen_linear_attention_hip_backward(t["do"], t["q"], t["k"], t["v"], t["g"], cu)
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a, b)
+
+
+def test_offsets_that_do_not_ascend_stay_inside_the_tensors():
+    """Clamped to [0, total]; what comes out is not specified."""
+    from scree_amd.kernels.hip import varlen_linear_attention_hip, varlen_linear_attention_hip_backward
+
+    for offsets in ([0, 300, 100, 400], [0, -7, 900, 400], [250, 0, 0, 400], [400, 400, 400, 0]):
+        say(f"case: offsets {offsets}")
+        cu = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+        t = _inputs([400], 4, 2, 64, 64, torch.bfloat16, 5, False, True)
+        s0 = randn((3, 2, 64, 64), torch.float32, 6)
+        room = torch.full((600, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, initial_state=s0, return_state=True,
+                                    out=room[100:500])
+        varlen_linear_attention_hip_backward(t["do"], t["q"], t["k"], t["v"], t["g"], cu, initial_state=s0, dstate=s0)
+        torch.cuda.synchronize()
+        assert (room[:100] == 7).all() and (room[500:] == 7).all()
+
+
+def test_non_finite_values_stay_in_their_sequence_and_head():
+    from scree_amd.kernels.hip import varlen_linear_attention_hip, varlen_linear_attention_hip_backward
+
+    lengths = [200, 90, 300]
+    _, cu = cu_of(lengths)
+    t = _inputs(lengths, 4, 2, 64, 64, torch.bfloat16, 5, False, True)
+    t["v"][250, 1, 3], t["k"][260, 1, 5] = float("nan"), float("inf")
+    o = varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu)
+    grads = varlen_linear_attention_hip_backward(t["do"], t["q"], t["k"], t["v"], t["g"], cu)[:3]
+    hit = torch.zeros(590, dtype=torch.bool, device="cuda")
+    hit[200:290] = True
+    assert torch.isnan(o[250:290, 2:, 3]).all()
+    for x in (o, *grads):
+        half = x.shape[1] // 2
+        assert torch.isfinite(x[~hit]).all() and torch.isfinite(x[:, :half]).all()
+
+
+def test_backward_twice_and_broadcast_heads():
+    """A retained graph gives the same gradients again; K/V heads expanded from
+    one sum theirs."""
+    from scree_amd.kernels.hip import varlen_linear_attention_hip
+
+    lengths = [500, 40]
+    _, cu = cu_of(lengths)
+    t = _inputs(lengths, 4, 4, 64, 64, torch.float32, 5, False, True)
+    one = [t[x][:, :1].clone().requires_grad_(True) for x in ("k", "v")]
+    q = t["q"].clone().requires_grad_(True)
+    g = torch.full((4,), -0.1, device="cuda")
+    o = varlen_linear_attention_hip(q, *[x.expand(-1, 4, -1) for x in one], g, cu)
+    first = torch.autograd.grad(o, [q, *one], t["do"], retain_graph=True)
+    for a, b in zip(first, torch.autograd.grad(o, [q, *one], t["do"])):
+        assert torch.equal(a, b)
+    # against four query heads on one K/V head
+    o1 = varlen_linear_attention_hip(q, *one, g[:1], cu)
+    assert torch.equal(o, o1)
+    want = torch.autograd.grad(o1, [q, *one], t["do"])
+    bound, _ = _bounds(torch.float32, lengths, {**t, "k": t["k"][:, :1], "v": t["v"][:, :1], "g": g[:1]}, 0.125)
+    for name, a, b in zip(("dq", "dk", "dv"), first, want):
+        check_close(name, np64(a), np64(b), 2 * bound[name] + 8 * EPS * np.abs(np64(b)))
+
+
+def test_on_another_stream():
+    from scree_amd.kernels.hip import linear_attention_step_hip, varlen_linear_attention_hip
+
+    lengths = [300, 40]
+    _, cu = cu_of(lengths)
+    t = _inputs(lengths, 4, 2, 64, 64, torch.bfloat16, 5, True, True)
+    want = varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, initial_state=t["s0"], return_state=True)
+    step = linear_attention_step_hip(t["q"][:2], t["k"][:2], t["v"][:2], t["g"], t["s0"].clone())
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, initial_state=t["s0"], return_state=True)
+        got_step = linear_attention_step_hip(t["q"][:2], t["k"][:2], t["v"][:2], t["g"], t["s0"].clone())
+    side.synchronize()
+    for a, b in zip((*got, got_step), (*want, step)):
+        assert torch.equal(a, b)

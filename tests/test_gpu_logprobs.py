@@ -229,7 +229,8 @@ def test_graph_replays_match_eager_without_host_sync():
 
     def step():
         out = varlen_token_logprobs_hip(buf, y, 8)
-        return (*out, *torch.autograd.grad(out[:3], [buf], g))
+        dx, = torch.autograd.grad(out[:3], [buf], g)
+        return tuple(t.detach() for t in out) + (dx,)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -250,3 +251,41 @@ def test_graph_replays_match_eager_without_host_sync():
         torch.cuda.synchronize()
         for a, b in zip(captured, want):
             assert torch.equal(a, b)
+
+
+def test_rows_past_2_31_elements():
+    from scree_amd.kernels.hip import varlen_token_logprobs_hip
+
+    small, y = _logits(3, 5000, torch.bfloat16, 12)
+    far = torch.empty((2 * ((1 << 30) + 3) + 5000,), dtype=torch.bfloat16, device="cuda")
+    view = far.as_strided((3, 5000), ((1 << 30) + 3, 1))
+    view.copy_(small)
+    for a, b in zip(varlen_token_logprobs_hip(view, y, 7), varlen_token_logprobs_hip(small, y, 7)):
+        assert torch.equal(a, b)
+    g = randn((3,), torch.float32, 1)
+    leaf, near = view.detach().requires_grad_(True), small.clone().requires_grad_(True)
+    got, = torch.autograd.grad(varlen_token_logprobs_hip(leaf, y).logprob, [leaf], g)
+    want, = torch.autograd.grad(varlen_token_logprobs_hip(near, y).logprob, [near], g)
+    assert torch.equal(got, want)
+
+
+def test_large_logits_take_streaming_loads():
+    """Past 256 MB the loads change; 70,000 rows of 4,001 fp16 are 560 MB."""
+    from scree_amd.kernels.hip import varlen_token_logprobs_hip
+
+    x = torch.randn((70000, 4001), device="cuda", dtype=torch.float16)
+    y = torch.randint(0, 4001, (70000,), device="cuda")
+    leaf = x.requires_grad_(True)
+    out = varlen_token_logprobs_hip(leaf, y, 3)
+    g = torch.randn(70000, device="cuda")
+    dx, = torch.autograd.grad(out.logprob, [leaf], g)
+    rows = slice(40000, 40007)
+    part = x.detach()[rows].clone().requires_grad_(True)
+    want = varlen_token_logprobs_hip(part, y[rows], 3)
+    # the same sums in another order (few rows are split): both within E of exact
+    E = (4001 / 256 + 80) * EPS
+    assert torch.equal(out.top_index[rows], want.top_index)
+    assert (out.logprob[rows] - want.logprob).abs().max() <= 2 * (E + 2 * EPS * 30)
+    dw, = torch.autograd.grad(want.logprob, [part], g[rows])
+    # each is one rounding of values E apart: 2 u and 2 E of themselves, and a subnormal's step
+    assert ((dx[rows].float() - dw.float()).abs() <= 2 * (2.0 ** -11 + E) * dw.float().abs() + 2.0 ** -24).all()
