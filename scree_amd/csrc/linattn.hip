@@ -333,9 +333,7 @@ constexpr int walk_waves() {
   return w < 1 ? 1 : w > most ? most : w;
 }
 
-// NW waves; wave w owns columns [16 w, 16 w + 16) of z, out and the state.
-// Two waves to a SIMD with 32 columns each (half the LDS reads, twice the
-// registers) ran 1.5x longer: what bounds the walk is waiting.
+// NW waves; wave w owns columns [16 NT w, 16 NT (w + 1)) of z, out and the state.
 // XLOOP: x's heads of a group in turn (x_loop > 1).
 template <typename T, int DX, int NW, int NT, bool OUT, bool XLOOP>
 __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void lin_walk_kernel(WalkArgs a) {
@@ -829,7 +827,8 @@ struct StepArgs {
   int kv_heads, group, dk, dv;
   float scale;
 };
-template <typename T, int ROWS>  // ROWS * 32 >= dk
+// NT: the new states are stored past the caches (kStepNtBytes).
+template <typename T, int ROWS, bool NT>  // ROWS * 32 >= dk
 __global__ __launch_bounds__(kStepThreads) void lin_step_kernel(StepArgs a) {
   __shared__ float qs[ROWS * 32];
   __shared__ float4 part[kStepThreads / 64][8];
@@ -869,7 +868,8 @@ __global__ __launch_bounds__(kStepThreads) void lin_step_kernel(StepArgs a) {
     st[i].y = fmaf(lam, st[i].y, kd * vv[1]);
     st[i].z = fmaf(lam, st[i].z, kd * vv[2]);
     st[i].w = fmaf(lam, st[i].w, kd * vv[3]);
-    *reinterpret_cast<float4*>(so + (int64_t)d * a.dv) = st[i];
+    if constexpr (NT) st16_nt(so + (int64_t)d * a.dv, __builtin_bit_cast(uint4, st[i]));
+    else *reinterpret_cast<float4*>(so + (int64_t)d * a.dv) = st[i];
   }
   for (int h = 0; h < a.group; ++h) {
     const int head = kvh * a.group + h;
@@ -1014,23 +1014,27 @@ int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)items), dim3(64 * NW), lds, stream, a);
   return check_launch(fn);
 }
+// 32 columns to a wave instead of 16 halve the LDS reads of a walk and keep two
+// waves on a SIMD instead of four.  With 16-bit states of 128 rows and enough
+// walks to fill the GPU that is faster (config 5's forward 719 us against 838,
+// 16 x 1,000 tokens of 16 heads 118 against 131); with few walks, where each
+// one's time counts, or fewer rows it is slower (1 x 500 tokens 25 us against 23,
+// 16 x 1,000 tokens of 16 x 64 70 against 62).
+constexpr int64_t kWideWalks = 320;
 template <typename T, bool OUT, bool XLOOP, int DX>
 int walk_z(const char* fn, const WalkArgs& a, int roles, hipStream_t stream) {
   const int dz = a.role[0].dz;
 #define WALK(NW, NT) return launch_walk<T, DX, NW, NT, OUT, XLOOP>(fn, a, roles, stream)
-  if constexpr (OUT && sizeof(T) == 2 && DX <= 128) {
-    if constexpr (DX <= 32)
-      if (dz <= 32) WALK(1, 2);
-    if constexpr (DX <= 64)
-      if (dz <= 64) WALK(2, 2);
-    WALK(4, 2);
-  } else {
-    if constexpr (DX <= 64)
-      if (dz <= 32) WALK(2, 1);
-    if constexpr (DX <= 128)
-      if (DX <= 32 || dz <= 64) WALK(4, 1);
-    if constexpr (DX > 32) WALK(8, 1);
+  if constexpr (DX <= 64)
+    if (dz <= 32) WALK(2, 1);
+  if constexpr (OUT && sizeof(T) == 2 && DX == 128) {
+    int64_t groups = 0;
+    for (int i = 0; i < roles; ++i) groups += (int64_t)a.slots * a.kv_heads * (a.role[i].x_group / a.role[i].x_loop);
+    if (dz > 64 && groups > kWideWalks) WALK(4, 2);
   }
+  if constexpr (DX <= 128)
+    if (DX <= 32 || dz <= 64) WALK(4, 1);
+  if constexpr (DX > 32) WALK(8, 1);
 #undef WALK
 }
 // One launch for `roles` walks of equal dims, all with x_loop > 1 or none.
@@ -1146,17 +1150,23 @@ int run_bwd(const char* fn, const Shape& s, const void* dout, const void* q, con
   return walk_out<T>(fn, a, 1, stream);
 }
 
+// States that do not fit the 256 MB behind the L2s, old and new, are not kept
+// there for the next step: 256 rows of 8 x 128 x 128 take 54 us with streaming
+// stores, 61 without.
+constexpr int64_t kStepNtBytes = 256ll << 20;
 template <typename T>
 int run_step(const char* fn, const StepArgs& a, int64_t rows, hipStream_t stream) {
   const int64_t items = rows * a.kv_heads * ((a.dv + 31) / 32);
   if (items * kStepThreads > 0xffffffffll)
     return set_error(SCREE_ERR_INVALID, "%s: %lld workgroups are too many", fn, (long long)items);
-  const dim3 grid((unsigned)items);
+  const int64_t states = rows * a.kv_heads * a.dk * a.dv * 4;
+  const bool nt = (a.state == a.state_out ? 1 : 2) * states >= kStepNtBytes;
   const int need = (a.dk + 31) / 32;
-  if (need <= 1) hipLaunchKernelGGL((lin_step_kernel<T, 1>), grid, dim3(kStepThreads), 0, stream, a);
-  else if (need <= 2) hipLaunchKernelGGL((lin_step_kernel<T, 2>), grid, dim3(kStepThreads), 0, stream, a);
-  else if (need <= 4) hipLaunchKernelGGL((lin_step_kernel<T, 4>), grid, dim3(kStepThreads), 0, stream, a);
-  else hipLaunchKernelGGL((lin_step_kernel<T, 8>), grid, dim3(kStepThreads), 0, stream, a);
+  auto kernel = need <= 1 ? (nt ? lin_step_kernel<T, 1, true> : lin_step_kernel<T, 1, false>)
+              : need <= 2 ? (nt ? lin_step_kernel<T, 2, true> : lin_step_kernel<T, 2, false>)
+              : need <= 4 ? (nt ? lin_step_kernel<T, 4, true> : lin_step_kernel<T, 4, false>)
+                          : (nt ? lin_step_kernel<T, 8, true> : lin_step_kernel<T, 8, false>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)items), dim3(kStepThreads), 0, stream, a);
   return check_launch(fn);
 }
 
