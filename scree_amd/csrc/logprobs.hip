@@ -163,17 +163,31 @@ struct LogprobOut {
   int64_t* top_index;
 };
 
-// A row's results from its merged statistics; called by one whole wave.
+// A row's given token and its logit: read first, so that nothing waits for
+// them at the end.
+struct Target {
+  int64_t at;
+  float logit;
+};
 template <typename T>
-__device__ __forceinline__ void finish_row(const Stats& a, const TopList& l, const T* __restrict__ x,
-                                           int64_t target, int vocab, int top_k, int64_t row,
-                                           const LogprobOut& out) {
+__device__ __forceinline__ Target read_target(const void* targets, int target_bytes, const T* x, int vocab,
+                                              int64_t row) {
+  Target t;
+  t.at = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row]
+                           : (int64_t)static_cast<const int32_t*>(targets)[row];
+  t.logit = t.at >= 0 && t.at < vocab ? to_f32(x[t.at]) : 0.f;
+  return t;
+}
+
+// A row's results from its merged statistics; called by one whole wave.
+__device__ __forceinline__ void finish_row(const Stats& a, const TopList& l, const Target& target,
+                                           int vocab, int top_k, int64_t row, const LogprobOut& out) {
   const int lane = threadIdx.x & 63;
   const float ls = logf(a.s);
   if (lane == 0) {
     float lp = 0.f;  // a row without a target
-    if (target >= vocab) lp = __builtin_nanf("");
-    else if (target >= 0) lp = (to_f32(x[target]) - a.m) - ls;
+    if (target.at >= vocab) lp = __builtin_nanf("");
+    else if (target.at >= 0) lp = (target.logit - a.m) - ls;
     out.logprob[row] = lp;
     out.entropy[row] = ls - a.t / a.s;
     if (out.stats) {
@@ -201,6 +215,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
   const T* x = logits + row * stride;
   const int c0 = part * part_cols, c1 = min(vocab, c0 + part_cols);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Target target = {-1, 0.f};
+  if (parts == 1 && wave == 0) target = read_target(targets, target_bytes, x, vocab, row);
 
   Stats a = {-__builtin_inff(), 0.f, 0.f};
   TopList l;
@@ -305,9 +321,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
       part_top[(int64_t)blockIdx.x * top_k + lane] = make_float2(l.v, __builtin_bit_cast(float, l.i));
     return;
   }
-  const int64_t target = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row]
-                                           : (int64_t)static_cast<const int32_t*>(targets)[row];
-  finish_row<T>(a, l, x, target, vocab, top_k, row, out);
+  finish_row(a, l, target, vocab, top_k, row, out);
 }
 
 // One wave per row joins the parts' statistics and lists.
@@ -318,6 +332,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(
     const float2* __restrict__ part_top, LogprobOut out) {
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x;
+  const Target target = read_target(targets, target_bytes, logits + row * stride, vocab, row);
   Stats a = {-__builtin_inff(), 0.f, 0.f};
   for (int p = lane; p < parts; p += 64) {
     const float* ps = part_stats + 3 * (row * parts + p);
@@ -344,9 +359,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(
       for (int i = 0; i < R; ++i) offer(l, c[i].x, __builtin_bit_cast(int, c[i].y), top_k);
     }
   }
-  const int64_t target = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row]
-                                           : (int64_t)static_cast<const int32_t*>(targets)[row];
-  finish_row<T>(a, l, logits + row * stride, target, vocab, top_k, row, out);
+  finish_row(a, l, target, vocab, top_k, row, out);
 }
 
 // --------------------------------------------------------------- backward
