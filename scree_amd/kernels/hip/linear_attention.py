@@ -100,45 +100,65 @@ def workspace_bytes(batch, total, heads, kv_heads, k_dim, v_dim, backward):
                                                             v_dim, int(backward)))
 
 
-def _workspace(cu, q, k, v, backward):
-    n = workspace_bytes(cu.numel() - 1, q.shape[0], q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-                        backward)
-    return (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None), n
-
-
 def _strides(ts, extra=()):
     return _ffi.int64_array(sum([_row_head(t) for t in ts], ()) + extra)
+
+
+def _like(t):
+    """A fresh contiguous tensor of ``t``'s shape."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _new_state(cu, k, v):
+    return torch.empty((cu.numel() - 1, *k.shape[1:], v.shape[2]), dtype=torch.float32,
+                       device=k.device)
+
+
+def _sizes(q, k, v, cu):
+    n, h, dk = q.shape
+    return cu.numel() - 1, n, h, k.shape[1], dk, v.shape[2]
 
 
 def linear_fwd(q, k, v, log_decay, cu, scale, init, want_state, out):
     """``(final states or None, workspace or None)``; the backward of the same
     call can take the workspace's states."""
-    batch = cu.numel() - 1
-    last = None
-    if want_state:
-        last = torch.empty((batch, k.shape[1], k.shape[2], v.shape[2]), dtype=torch.float32,
-                           device=q.device)
-    ws, nws = _workspace(cu, q, k, v, False)
+    last = _new_state(cu, k, v) if want_state else None
+    sizes = _sizes(q, k, v, cu)
+    nws = workspace_bytes(*sizes, False)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
     _ffi.launch(_ffi.lib().scree_linear_attn_fwd, q, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 log_decay.data_ptr(), out.data_ptr(), _ffi.ptr(init), _ffi.ptr(last), cu.data_ptr(),
-                batch, q.shape[0], q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-                _strides((q, k, v, out)), scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
+                *sizes, _strides((q, k, v, out)), scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
     return last, ws
 
 
-def linear_bwd(do, q, k, v, log_decay, cu, scale, init, dlast, want_dinit, fwd_ws=None):
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    batch = cu.numel() - 1
-    dinit = None
-    if want_dinit:
-        dinit = torch.empty((batch, k.shape[1], k.shape[2], v.shape[2]), dtype=torch.float32,
-                            device=q.device)
-    ws, nws = _workspace(cu, q, k, v, fwd_ws is None)
+# The backward runs on autograd's own thread, where Python costs several times
+# what it does here: what the forward knows of the call (sizes, the strides of
+# a contiguous gradient) is laid out by it.
+def _bwd_plan(q, k, v, cu):
+    n, h, _ = q.shape
+    dv = v.shape[2]
+    rows = [_row_head(t) for t in (q, k, v)]
+    fresh = [(t.shape[1] * t.shape[2], t.shape[2]) for t in (q, k, v)]
+    return (_sizes(q, k, v, cu),
+            _ffi.int64_array(sum([(h * dv, dv), *rows, *fresh], ())),
+            _ffi.dtype_code(q.dtype))
+
+
+def linear_bwd(do, q, k, v, log_decay, cu, scale, init, dlast, want_dinit, fwd_ws=None, plan=None):
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    dinit = _new_state(cu, k, v) if want_dinit else None
+    sizes, strides, code = _bwd_plan(q, k, v, cu) if plan is None else plan
+    if not do.is_contiguous():
+        strides = _strides((do, q, k, v, dq, dk, dv))
+    nws = workspace_bytes(*sizes, fwd_ws is None)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
     _ffi.launch(_ffi.lib().scree_linear_attn_bwd, q, do.data_ptr(), q.data_ptr(), k.data_ptr(),
                 v.data_ptr(), log_decay.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                _ffi.ptr(init), _ffi.ptr(dlast), _ffi.ptr(dinit), _ffi.ptr(fwd_ws), cu.data_ptr(), batch,
-                q.shape[0], q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-                _strides((do, q, k, v, dq, dk, dv)), scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
+                _ffi.ptr(init), _ffi.ptr(dlast), _ffi.ptr(dinit), _ffi.ptr(fwd_ws), cu.data_ptr(),
+                *sizes, strides, scale, code, _ffi.ptr(ws), nws)
     return dq, dk, dv, dinit
 
 
@@ -151,6 +171,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         last, ws = linear_fwd(qk, kk, vk, log_decay, cu, scale, s0, want_state, out)
         ctx.save_for_backward(qk, kk, vk, log_decay, cu, s0, ws)
         ctx.scale = scale
+        ctx.plan = _bwd_plan(qk, kk, vk, cu)
         ctx.set_materialize_grads(False)
         return (out, last) if want_state else out
 
@@ -162,7 +183,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         if do is None:
             do = torch.zeros((*q.shape[:2], v.shape[2]), dtype=q.dtype, device=q.device)
         dq, dk, dv, dinit = linear_bwd(_view(do), q, k, v, log_decay, cu, ctx.scale, s0,
-                                       _state(dlast), ctx.needs_input_grad[6], ws)
+                                       _state(dlast), ctx.needs_input_grad[6], ws, ctx.plan)
         return dq, dk, dv, None, None, None, dinit, None
 
 

@@ -78,12 +78,15 @@ def _grad_of(g, shape):
     if g is None:
         return None
     assert g.shape == shape, f"a gradient must have its output's shape {tuple(shape)}"
+    if g.dtype == torch.float32 and g.is_contiguous():
+        return g
     return g.float().contiguous()
 
 
 def logprobs_bwd(x, targets, stats, entropy, top_i, dlogprob, dentropy, dtop):
     rows, vocab = x.shape
-    dx = torch.empty((rows, vocab), dtype=x.dtype, device=x.device)
+    dx = (torch.empty_like(x) if x.is_contiguous()
+          else torch.empty((rows, vocab), dtype=x.dtype, device=x.device))
     top_k = 0 if top_i is None else top_i.shape[1]
     grads = [_grad_of(dlogprob, (rows,)), _grad_of(dentropy, (rows,)), _grad_of(dtop, (rows, top_k))]
     if rows:
