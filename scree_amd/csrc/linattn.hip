@@ -371,23 +371,33 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
   const int c = lane & 15, g = lane >> 4;
   const int z0 = slice * DZ, zcols = min(DZ, r.dz - z0);
 
-  if constexpr (OUT) {
-    // rows behind the last sequence: the last slot's workgroups
-    if (r.zero_tail && slot == a.slots - 1) {
-      const int per = zcols / 8;
-      const int64_t tail = offset_at(a.cu, a.batch, a.total);
-      for (int h = 0; h < x_loop; ++h) {
-        T* out = static_cast<T*>(r.out) + (head + h) * r.o_head + z0;
-        for (int64_t q = threadIdx.x; q < (a.total - tail) * per; q += THREADS) {
-          T* p = out + (tail + q / per) * r.o_row + (int)(q % per) * 8;
-          st16(p, make_uint4(0u, 0u, 0u, 0u));
-          if constexpr (sizeof(T) == 4) st16(p + 4, make_uint4(0u, 0u, 0u, 0u));
-        }
+  // Rows behind the last sequence.  The slots from that of a sequence after the
+  // last one on have no segment (at least one for every seg such rows): they take
+  // a share each.  Where there is none, the last slot's workgroups take the rows.
+  [[maybe_unused]] auto zero_tail = [&](bool shared) {
+    const int64_t tail = offset_at(a.cu, a.batch, a.total);
+    const int past = (int)((uint32_t)tail / (uint32_t)a.seg) + a.batch;
+    if (shared ? slot < past : past < a.slots) return;
+    const int64_t shares = shared ? a.slots - past : 1, share = shared ? slot - past : 0;
+    const int64_t from = tail + (a.total - tail) * share / shares, to = tail + (a.total - tail) * (share + 1) / shares;
+    const int per = zcols / 8;
+    for (int h = 0; h < x_loop; ++h) {
+      T* out = static_cast<T*>(r.out) + (head + h) * r.o_head + z0;
+      for (int64_t q = threadIdx.x; q < (to - from) * per; q += THREADS) {
+        T* p = out + (from + q / per) * r.o_row + (int)(q % per) * 8;
+        st16(p, make_uint4(0u, 0u, 0u, 0u));
+        if constexpr (sizeof(T) == 4) st16(p + 4, make_uint4(0u, 0u, 0u, 0u));
       }
     }
-  }
+  };
+  if constexpr (OUT)
+    if (r.zero_tail && slot == a.slots - 1) zero_tail(false);
   Segment sg;
-  if (!find_segment(a.cu, a.batch, a.total, a.seg, slot, sg)) return;
+  if (!find_segment(a.cu, a.batch, a.total, a.seg, slot, sg)) {
+    if constexpr (OUT)
+      if (r.zero_tail) zero_tail(true);
+    return;
+  }
   const bool back = r.reverse;
   const int first = back ? sg.count - 1 : 0, final = sg.count - 1 - first;
   // a segment whose state nobody reads
@@ -566,9 +576,20 @@ __global__ __launch_bounds__(64 * NW, (walk_waves<T, DX, NW, NT, OUT>())) void l
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(st[m][u][i]));
             if (__ballot(top > 32768.f)) {
+              // the largest finite one: an infinity stays with its own column
+              top = 0.f;
+#pragma unroll
+              for (int m = 0; m < DX / 16; ++m)
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const float f = fabsf(st[m][u][i]);
+                    top = fmaxf(top, f < __builtin_inff() ? f : 0.f);
+                  }
 #pragma unroll
               for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-              const int over = __builtin_amdgcn_frexp_expf(top) - 15;
+              const int over = max(__builtin_amdgcn_frexp_expf(top) - 15, 0);
               up = __builtin_amdgcn_ldexpf(1.f, over);
               const float down = __builtin_amdgcn_ldexpf(1.f, -over);
 #pragma unroll
@@ -921,8 +942,8 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // 412 us in segments of 2,048, 463 in 1,024 and 527 in 512, and the fewer
 // segments the less traffic of their states (64 KB each, read and written five
 // times).  At least kLinMinSeg, at most kLinMaxSeg, so that one long sequence
-// among many heads does not outlast the rest (config 5: 2,667 us at 4,096,
-// 2,818 at 2,048).  A small batch of short sequences is one segment each: two
+// among many heads does not outlast the rest (a training step of 83,977 tokens
+// of 32 x 128: 2,667 us at 4,096, 2,818 at 2,048).  A small batch of short sequences is one segment each: two
 // launches less (22 us against 29 at 1,980 tokens of 16 sequences).
 constexpr int64_t kLinFill = 512;
 constexpr int kLinMinSeg = 128, kLinMaxSeg = 4096;
@@ -1016,7 +1037,7 @@ int launch_walk(const char* fn, WalkArgs a, int roles, hipStream_t stream) {
 }
 // 32 columns to a wave instead of 16 halve the LDS reads of a walk and keep two
 // waves on a SIMD instead of four.  With 16-bit states of 128 rows and enough
-// walks to fill the GPU that is faster (config 5's forward 719 us against 838,
+// walks to fill the GPU that is faster (83,977 tokens of 32 x 128 forward 719 us against 838,
 // 16 x 1,000 tokens of 16 heads 118 against 131); with few walks, where each
 // one's time counts, or fewer rows it is slower (1 x 500 tokens 25 us against 23,
 // 16 x 1,000 tokens of 16 x 64 70 against 62).
@@ -1231,8 +1252,9 @@ extern "C" int scree_linear_attn_bwd(const void* dout, const void* q, const void
     return set_error(SCREE_ERR_INVALID, "%s: cu_seqlens, log_decay or strides is null", fn);
   const void* states[] = {initial_state, dfinal_state, dinitial_state, fwd_workspace};
   if (int rc = check_states(fn, states, 4)) return rc;
-  if (scale == 0.f || !(scale - scale == 0.f))
-    return set_error(SCREE_ERR_INVALID, "%s: scale must be finite and not zero", fn);
+  const float inv = 1.f / scale;  // run_bwd carries R / scale
+  if (!(scale - scale == 0.f) || !(inv - inv == 0.f))
+    return set_error(SCREE_ERR_INVALID, "%s: scale %g must be finite, and 1 / scale too", fn, (double)scale);
   if (total_tokens) {
     const Arg args[] = {{"dout", dout, strides, v_dim}, {"q", q, strides + 2, k_dim},
                         {"k", k, strides + 4, k_dim}, {"v", v, strides + 6, v_dim},

@@ -23,8 +23,10 @@ import functools
 import math
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _ffi
+from ._once import once
 from .attention import _MAX_STRIDE, _cu
 
 MAX_DIM = 256
@@ -84,6 +86,19 @@ def _view(t):
                 and t.shape[2] <= s0 < _MAX_STRIDE):
             return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _out(out, shape, q, what):
+    """``(out, where the library writes it)``, ``out`` checked or a new tensor."""
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        return out, out
+    assert out.shape == shape and out.dtype == q.dtype and out.device == q.device, (
+        f"out must be ({what}, heads, v_dim) like q")
+    assert out.is_contiguous() or 0 not in out.stride(), "out must not be an expanded tensor"
+    # autograd sees the write, as that of any in-place operation
+    increment_version(out)
+    return out, _view(out)
 
 
 def _state(s):
@@ -182,8 +197,9 @@ class _LinearAttentionFn(torch.autograd.Function):
             return (None,) * 8
         if do is None:
             do = torch.zeros((*q.shape[:2], v.shape[2]), dtype=q.dtype, device=q.device)
-        dq, dk, dv, dinit = linear_bwd(_view(do), q, k, v, log_decay, cu, ctx.scale, s0,
-                                       _state(dlast), ctx.needs_input_grad[6], ws, ctx.plan)
+        grads = linear_bwd(_view(do), q, k, v, log_decay, cu, ctx.scale, s0, _state(dlast),
+                           ctx.needs_input_grad[6], ws, ctx.plan)
+        dq, dk, dv, dinit = once("varlen linear attention", *grads)
         return dq, dk, dv, None, None, None, dinit, None
 
 
@@ -220,13 +236,7 @@ def varlen_linear_attention_hip(q, k, v, log_decay, cu_seqlens, scale=None, init
         assert out is None, "out= is not supported when an input requires grad"
         return _LinearAttentionFn.apply(q, k, v, log_decay.contiguous(), cu, scale, initial_state,
                                         bool(return_state))
-    shape = (*q.shape[:2], v.shape[2])
-    if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    else:
-        assert out.shape == shape and out.dtype == q.dtype and out.device == q.device, (
-            "out must be (total_tokens, heads, v_dim) like q")
-    ok = _view(out)
+    out, ok = _out(out, (*q.shape[:2], v.shape[2]), q, "total_tokens")
     last, _ = linear_fwd(_view(q), _view(k), _view(v), log_decay.contiguous(), cu, scale,
                          _state(initial_state), return_state, ok)
     if ok is not out:
@@ -285,14 +295,11 @@ def linear_attention_step_hip(q, k, v, log_decay, state, scale=None, state_out=N
         state_out, rows_out = state, rows
     else:
         rows_out = _step_state(state_out, "state_out", b, k, v)
-    if out is None:
-        out = torch.empty((b, h, dv), dtype=q.dtype, device=q.device)
-    else:
-        assert out.shape == (b, h, dv) and out.dtype == q.dtype and out.device == q.device, (
-            "out must be (batch, heads, v_dim) like q")
+    out, ok = _out(out, (b, h, dv), q, "batch")
     if b == 0:
         return out
-    qk, kk, vk, ok = _view(q), _view(k), _view(v), _view(out)
+    increment_version(state_out)
+    qk, kk, vk = _view(q), _view(k), _view(v)
     _ffi.launch(_ffi.lib().scree_linear_attn_step, qk, qk.data_ptr(), kk.data_ptr(), vk.data_ptr(),
                 log_decay.contiguous().data_ptr(), ok.data_ptr(), state.data_ptr(),
                 state_out.data_ptr(), b, h, hk, dk, dv, _strides((qk, kk, vk, ok), (rows, rows_out)),

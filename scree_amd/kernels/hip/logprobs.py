@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _ffi
+from ._once import once
 
 MAX_TOP_K = 64
 
@@ -74,10 +75,11 @@ def logprobs_fwd(x, targets, top_k, want_stats):
     return logprob, entropy, stats, top_lp, top_i
 
 
-def _grad_of(g, shape):
+def _grad_of(g, shape, x):
     if g is None:
         return None
     assert g.shape == shape, f"a gradient must have its output's shape {tuple(shape)}"
+    assert g.get_device() == x.get_device(), "a gradient must be on the same device as logits"
     if g.dtype == torch.float32 and g.is_contiguous():
         return g
     return g.float().contiguous()
@@ -88,7 +90,8 @@ def logprobs_bwd(x, targets, stats, entropy, top_i, dlogprob, dentropy, dtop):
     dx = (torch.empty_like(x) if x.is_contiguous()
           else torch.empty((rows, vocab), dtype=x.dtype, device=x.device))
     top_k = 0 if top_i is None else top_i.shape[1]
-    grads = [_grad_of(dlogprob, (rows,)), _grad_of(dentropy, (rows,)), _grad_of(dtop, (rows, top_k))]
+    grads = [_grad_of(dlogprob, (rows,), x), _grad_of(dentropy, (rows,), x),
+             _grad_of(dtop, (rows, top_k), x)]
     if rows:
         _ffi.launch(_ffi.lib().scree_token_logprobs_bwd, x, x.data_ptr(), x.stride(0),
                     targets.data_ptr(), targets.element_size(), rows, vocab, top_k,
@@ -114,7 +117,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
     def backward(ctx, dlogprob, dentropy, dtop=None, _=None):
         if dlogprob is None and dentropy is None and dtop is None:
             return None, None, None
-        return logprobs_bwd(*ctx.saved_tensors, dlogprob, dentropy, dtop), None, None
+        dx = logprobs_bwd(*ctx.saved_tensors, dlogprob, dentropy, dtop)
+        return *once("token log probabilities", dx), None, None
 
 
 def varlen_token_logprobs_hip(logits, targets, top_k: int = 0) -> TokenLogprobs:

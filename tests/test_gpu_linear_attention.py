@@ -472,3 +472,68 @@ def test_on_another_stream():
     side.synchronize()
     for a, b in zip((*got, got_step), (*want, step)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,rows,h,hk,d", [([300], 20000, 4, 2, 64), ([9000, 1, 0], 9001 + 40, 8, 1, 128),
+                                                 ([0, 0], 5000, 2, 2, 32), ([5000], 9000, 32, 8, 64)])
+def test_long_tails_become_zeros_in_the_gradients(dtype, lengths, rows, h, hk, d):
+    """Fewer rows than a segment behind the last sequence, and many segments' worth."""
+    from scree_amd.kernels.hip import varlen_linear_attention_hip_backward
+
+    n = sum(lengths)
+    _, cu = cu_of(lengths)
+    t = _inputs([rows], h, hk, d, d, dtype, 5, False, True)
+    for x in ("q", "k", "v", "do"):
+        t[x][n:] = float("nan")
+    junk = torch.full((4 * rows, h, d), float("nan"), device="cuda")  # what the gradients' memory held
+    del junk
+    grads = varlen_linear_attention_hip_backward(t["do"], t["q"], t["k"], t["v"], t["g"], cu)[:3]
+    for grad in grads:
+        assert (grad[n:] == 0).all() and torch.isfinite(grad).all()
+
+
+def test_an_infinite_state_column_stays_alone():
+    """An infinity in one column of an fp16 walk's state leaves the others' values."""
+    from scree_amd.kernels.hip import varlen_linear_attention_hip
+
+    lengths = [150, 20]
+    _, cu = cu_of(lengths)
+    t = _inputs(lengths, 4, 2, 64, 64, torch.float16, 5, True, False)
+    want, last = varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, initial_state=t["s0"], return_state=True)
+    s0 = t["s0"].clone()
+    s0[0, 1, 7, 5] = float("inf")
+    o, got = varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, initial_state=s0, return_state=True)
+    others = [c for c in range(64) if c != 5]
+    assert torch.equal(o[..., others], want[..., others]) and torch.equal(got[..., others], last[..., others])
+    assert not torch.isfinite(o[:150, 2:, 5]).any() and torch.equal(o[:, :2], want[:, :2])
+
+
+def test_in_place_writes_are_seen_by_autograd():
+    """A state or output that a recorded graph still needs is not changed unseen;
+    a second derivative is refused."""
+    from scree_amd.kernels.hip import linear_attention_step_hip, varlen_linear_attention_hip
+
+    _, cu = cu_of([5, 3])
+    t = _inputs([5, 3], 4, 2, 64, 32, torch.float32, 1, True, True)
+    q = t["q"].clone().requires_grad_(True)
+    o = varlen_linear_attention_hip(q, t["k"], t["v"], t["g"], cu, initial_state=t["s0"])
+    with torch.no_grad():
+        linear_attention_step_hip(t["q"][:2], t["k"][:2], t["v"][:2], t["g"], t["s0"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    w = torch.ones_like(t["do"], requires_grad=True)
+    buf = torch.empty_like(t["do"])
+    y = w * buf
+    varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(AssertionError, match="expanded"):
+        varlen_linear_attention_hip(t["q"], t["k"], t["v"], t["g"], cu, out=buf[:, :1].expand(-1, 4, -1))
+    grad, = torch.autograd.grad(varlen_linear_attention_hip(q, t["k"], t["v"], t["g"], cu).sum(), [q], create_graph=True)
+    with pytest.raises(NotImplementedError, match="second derivative"):
+        grad.sum().backward()
+    with torch.inference_mode():
+        s = t["s0"].clone()
+        linear_attention_step_hip(t["q"][:2], t["k"][:2], t["v"][:2], t["g"], s)
+        assert torch.equal(s, t["s0"]) is False

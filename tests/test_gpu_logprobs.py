@@ -220,6 +220,19 @@ def test_refusals_on_the_device():
             varlen_token_logprobs_hip(**args)
 
 
+def test_gradients_on_the_host_and_second_derivatives_are_refused():
+    from scree_amd.kernels.hip import varlen_token_logprobs_hip, varlen_token_logprobs_hip_backward
+
+    x, y = _logits(4, 50, torch.float32, 1)
+    for name, shape in (("dlogprob", (4,)), ("dentropy", (4,)), ("dtop_logprob", (4, 2))):
+        with pytest.raises(AssertionError, match="same device"):
+            varlen_token_logprobs_hip_backward(x, y, top_k=2, **{name: torch.zeros(shape)})
+    leaf = x.clone().requires_grad_(True)
+    grad, = torch.autograd.grad(varlen_token_logprobs_hip(leaf, y).logprob.sum(), [leaf], create_graph=True)
+    with pytest.raises(NotImplementedError, match="second derivative"):
+        grad.sum().backward()
+
+
 def test_graph_replays_match_eager_without_host_sync():
     from scree_amd.kernels.hip import varlen_token_logprobs_hip
 

@@ -136,7 +136,7 @@ def test_c_abi_refusals():
 
     assert bwd(dv=null) == _ffi.SCREE_ERR_INVALID and "dv is null" in err()
     assert bwd(fwd=odd) == _ffi.SCREE_ERR_INVALID and "aligned" in err()
-    for scale in (0.0, float("nan"), float("inf")):
+    for scale in (0.0, float("nan"), float("inf"), 1e-40):
         assert bwd(scale=scale) == _ffi.SCREE_ERR_INVALID and "scale" in err()
     # the forward's states at hand, half the room is enough
     assert bwd(n=100000, ws=p, nws=2 * need - 1) == _ffi.SCREE_ERR_WORKSPACE
