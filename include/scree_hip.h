@@ -308,8 +308,11 @@ int scree_varlen_softmax_bwd(const void* y, const void* dy, void* dx, const int3
  * output gets its operands in two (fp16) or three (bf16) terms.  The decay is
  * a constant of the head: it has no gradient.  Offsets must ascend; others
  * give unspecified values but never reach outside the tensors.  Rows of `o`
- * past the last sequence are left as they were.  No counterpart in the
- * reference. */
+ * past the last sequence are left as they were.  Outputs must not overlap
+ * inputs (a step's state in place apart).  log_decay is meant to be at most 0:
+ * growth can pass the range of 16-bit operands.  A NaN or infinity in a row of
+ * k or v may reach earlier outputs of its own sequence and head, at most 63
+ * rows before it.  No counterpart in the reference. */
 
 /* Bytes of workspace for the forward: the fp32 states between the segments
  * that long sequences are walked in; 0 when no sequence can have two.  The
@@ -331,8 +334,8 @@ int scree_linear_attn_fwd(const void* q, const void* k, const void* v, const flo
  * each group's query heads, without atomics.  Rows past the last sequence
  * become zeros.  `fwd_workspace` may be the workspace of the forward call with
  * the same q, k, v, log_decay, initial_state, offsets and sizes, left as that
- * call wrote it (it is only read), or NULL.  `scale` must be finite and not
- * zero.  In fp16 the rounded scores (scale * q.k here and in the forward,
+ * call wrote it (it is only read), or NULL.  `scale` and 1 / `scale` must be
+ * finite.  In fp16 the rounded scores (scale * q.k here and in the forward,
  * scale * do.v) overflow past 65504.  strides[14] = {dout, q, k, v, dq, dk, dv} x {row, head}. */
 int scree_linear_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
                           const float* log_decay, void* dq, void* dk, void* dv,

@@ -50,8 +50,17 @@ Pinning status of every function (how a plausible mistake would be caught):
 * ``schedule.build_schedule`` -- brute-force enumeration: every (sequence,
   block) appears exactly once, costs are non-increasing, ties broken by the
   stated key.
+* ``linear_attention.linear_attention_fwd`` -- an explicit double sum over
+  decayed ``(q_i . k_j) v_j`` per sequence, grouped heads and states included;
+  no counterpart in the reference.
+* ``linear_attention.linear_attention_bwd`` -- torch autograd through the same
+  recurrence in fp64 and central finite differences.
+* ``logprobs.token_logprobs`` -- ``torch.log_softmax``, ``torch.topk`` and the
+  entropy from them; ties, masked and non-finite rows by hand.
+* ``logprobs.token_logprobs_bwd`` -- central finite differences.
 
 No function is "parity unpinned".
 """
 
-from . import attention, core, norms, padding, schedule, softmax  # noqa: F401
+from . import (  # noqa: F401
+    attention, core, linear_attention, logprobs, norms, padding, schedule, softmax)

@@ -123,7 +123,8 @@ __device__ __forceinline__ void insert(TopList& l, float v, int i, int top_k) {
 // 64 lanes hold, at least top_k elements reach the top_k-th largest of those.
 // Found bit by bit in the upper half of the ordered bits, so at most 2^-7 of
 // its value below; the list then takes few more than top_k elements instead of
-// every new largest (16 rows x 128,000 with 20 alternatives: 54 -> 27 us).
+// every new largest (16 rows x 128,000 with 20 alternatives: 54 -> 27 us, and
+// 20 with the join's).
 template <int N>
 __device__ __forceinline__ void seed(TopList& l, const float (&mx)[N], int top_k) {
   uint32_t key[N];

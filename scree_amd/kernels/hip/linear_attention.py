@@ -220,13 +220,19 @@ def varlen_linear_attention_hip(q, k, v, log_decay, cu_seqlens, scale=None, init
     k_dim)`` and ``v`` ``(total_tokens, kv_heads, v_dim)`` share a dtype (fp16,
     bf16 or fp32); ``kv_heads`` divides ``heads`` and the dims are multiples of
     8 up to 256.  ``log_decay`` is fp32 ``(kv_heads,)``, ``log(lam)`` of each
-    head (0 for no decay).  ``cu_seqlens`` int32 ``(batch + 1,)`` offsets; an
+    head: 0 for no decay, -inf for none of the past; growth (above 0) can pass
+    the range of the 16-bit products' operands.  ``cu_seqlens`` int32 ``(batch + 1,)`` offsets; an
     empty sequence passes its state on.  ``scale`` defaults to
     ``1 / sqrt(k_dim)``.  ``initial_state`` fp32 ``(batch, kv_heads, k_dim,
     v_dim)`` continues earlier tokens; ``return_state`` also returns the
     states after the last tokens.  ``out`` is an optional preallocated output
-    (not when a gradient is recorded); rows past the last sequence are left as
-    they were.
+    (not when a gradient is recorded) that overlaps no input; rows past the last
+    sequence are left as they were.  A gradient needs a finite ``1 / scale``; it
+    has no derivative of its own.
+
+    In fp16 a score ``scale * q.k`` past 65504 overflows.  A NaN or infinity in a
+    token's k or v may reach earlier outputs of its own sequence and head, at
+    most 63 rows before it.
 
     Returns ``out`` ``(total_tokens, heads, v_dim)`` or ``(out, state)``.
     """
@@ -280,7 +286,7 @@ def linear_attention_step_hip(q, k, v, log_decay, state, scale=None, state_out=N
     ``(batch, kv_heads, v_dim)``; ``state`` fp32 ``(batch, kv_heads, k_dim,
     v_dim)``, rows of a larger pool of states allowed, becomes
     ``exp(log_decay) state + k v^T`` in place, or in ``state_out`` when given
-    (which must not overlap ``state``).  Returns ``scale * q state``
+    (which must not overlap ``state``, nor ``out`` any input).  Returns ``scale * q state``
     ``(batch, heads, v_dim)``; one step of what
     :func:`varlen_linear_attention_hip` computes.  No gradient is recorded.
     """
