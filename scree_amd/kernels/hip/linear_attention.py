@@ -32,9 +32,30 @@ from .attention import _MAX_STRIDE, _cu
 MAX_DIM = 256
 
 
-@functools.lru_cache(maxsize=256)
-def _shape_plan(qs, ks, vs, dtype):
-    """Checks that depend on shapes and dtype alone; ``(dtype code, default scale)``."""
+class _Plan:
+    """What a call's shapes, strides and dtypes decide; a loop asks for the same
+    one every step.  The arrays of strides are only read."""
+
+    __slots__ = ("code", "scale", "out_shape", "sizes", "in_place", "rows", "strides",
+                 "bwd_strides")
+
+    def __init__(self, qs, ks, vs, dtype, qst, kst, vst):
+        self.code = _ffi.dtype_code(dtype)
+        self.scale = 1.0 / math.sqrt(qs[2])
+        self.out_shape = (qs[0], qs[1], vs[2])
+        self.sizes = (qs[0], qs[1], ks[1], qs[2], vs[2])  # total, heads, kv_heads, k_dim, v_dim
+        # q, k and v are read where they lie (if they are aligned)
+        self.in_place = all(_readable(*x) for x in ((qs, qst), (ks, kst), (vs, vst)))
+        rows = _row_head(qs, qst) + _row_head(ks, kst) + _row_head(vs, vst)
+        o = (qs[1] * vs[2], vs[2])
+        fresh = tuple(x for t in (qs, ks, vs) for x in (t[1] * t[2], t[2]))
+        self.rows = rows + o
+        self.strides = _ffi.int64_array(self.rows)
+        self.bwd_strides = _ffi.int64_array(o + rows + fresh)
+
+
+@functools.lru_cache(maxsize=512)
+def _plan(qs, ks, vs, gs, dtype, kdtype, vdtype, gdtype, qst, kst, vst):
     assert len(qs) == len(ks) == len(vs) == 3, "q, k, v must be (tokens, heads, head_dim)"
     assert ks[:2] == vs[:2], "k and v must share tokens and heads"
     assert qs[0] == ks[0] and qs[2] == ks[2], "q and k must share tokens and head_dim"
@@ -43,18 +64,18 @@ def _shape_plan(qs, ks, vs, dtype):
     for d in (qs[2], vs[2]):
         assert 8 <= d <= MAX_DIM and d % 8 == 0, "head dims must be multiples of 8 up to 256"
     assert dtype in (torch.float16, torch.bfloat16, torch.float32), f"unsupported dtype {dtype}"
-    return _ffi.dtype_code(dtype), 1.0 / math.sqrt(qs[2])
+    assert dtype == kdtype == vdtype, "q, k, v must share a dtype"
+    assert gs == ks[1:2] and gdtype == torch.float32, "log_decay must be float32, one per K/V head"
+    return _Plan(qs, ks, vs, dtype, qst, kst, vst)
 
 
 def _check(q, k, v, log_decay):
     dev = q.get_device()
     assert dev >= 0, "linear attention on HIP requires ROCm device tensors"
-    plan = _shape_plan(q.shape, k.shape, v.shape, q.dtype)
-    assert q.dtype == k.dtype == v.dtype, "q, k, v must share a dtype"
+    plan = _plan(q.shape, k.shape, v.shape, log_decay.shape, q.dtype, k.dtype, v.dtype,
+                 log_decay.dtype, q.stride(), k.stride(), v.stride())
     assert dev == k.get_device() == v.get_device(), "q, k, v must be on the same device"
-    assert log_decay.shape == k.shape[1:2] and log_decay.dtype == torch.float32, (
-        "log_decay must be float32, one per K/V head")
-    assert log_decay.get_device() == dev, "log_decay must be on q's device"
+    assert dev == log_decay.get_device(), "log_decay must be on q's device"
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("log_decay is a constant of the head: it has no gradient here")
     return plan
@@ -67,31 +88,43 @@ def _check_state(s, name, batch, k, v):
     assert s.get_device() == k.get_device(), f"{name} must be on q's device"
 
 
-def _row_head(t):
+def _row_head(shape, stride):
     """Row and head strides; those of an axis of one are the contiguous ones."""
-    n, h, d = t.shape
-    s0, s1, _ = t.stride()
+    n, h, d = shape
+    s0, s1, _ = stride
     if h == 1:
         s1 = d
     return (h * d if n <= 1 else s0), s1
 
 
+def _readable(shape, stride):
+    """Whether the library can read these rows in place."""
+    n, h, d = shape
+    s0, s1 = _row_head(shape, stride)
+    if n == 0 or (stride[2] == 1 and s1 == d and s0 == h * d):
+        return True
+    return (stride[2] == 1 and s0 % 8 == 0 and s1 % 8 == 0 and 0 <= s1 < _MAX_STRIDE
+            and d <= s0 < _MAX_STRIDE)
+
+
 def _view(t):
     """``t`` itself when the library can read it in place, else an aligned copy."""
-    if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():
-            return t
-        s0, s1 = _row_head(t)
-        if (t.stride(2) == 1 and s0 % 8 == 0 and s1 % 8 == 0 and 0 <= s1 < _MAX_STRIDE
-                and t.shape[2] <= s0 < _MAX_STRIDE):
-            return t
+    if t.data_ptr() % 16 == 0 and _readable(t.shape, t.stride()):
+        return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _read(plan, q, k, v):
+    """q, k and v for the library, and whether the plan's strides are theirs."""
+    if plan.in_place and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        return q, k, v, True
+    return _view(q), _view(k), _view(v), False
 
 
 def _out(out, shape, q, what):
     """``(out, where the library writes it)``, ``out`` checked or a new tensor."""
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
         return out, out
     assert out.shape == shape and out.dtype == q.dtype and out.device == q.device, (
         f"out must be ({what}, heads, v_dim) like q")
@@ -116,77 +149,61 @@ def workspace_bytes(batch, total, heads, kv_heads, k_dim, v_dim, backward):
 
 
 def _strides(ts, extra=()):
-    return _ffi.int64_array(sum([_row_head(t) for t in ts], ()) + extra)
+    return _ffi.int64_array(sum([_row_head(t.shape, t.stride()) for t in ts], ()) + extra)
 
 
 def _like(t):
     """A fresh contiguous tensor of ``t``'s shape."""
     if t.is_contiguous():
         return torch.empty_like(t)
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return t.new_empty(t.shape)
 
 
-def _new_state(cu, k, v):
-    return torch.empty((cu.numel() - 1, *k.shape[1:], v.shape[2]), dtype=torch.float32,
-                       device=k.device)
+def _new_state(cu, plan, q):
+    _, _, hk, dk, dv = plan.sizes
+    return torch.empty((cu.numel() - 1, hk, dk, dv), dtype=torch.float32, device=q.device)
 
 
-def _sizes(q, k, v, cu):
-    n, h, dk = q.shape
-    return cu.numel() - 1, n, h, k.shape[1], dk, v.shape[2]
-
-
-def linear_fwd(q, k, v, log_decay, cu, scale, init, want_state, out):
+def linear_fwd(plan, planned, q, k, v, log_decay, cu, scale, init, want_state, out):
     """``(final states or None, workspace or None)``; the backward of the same
     call can take the workspace's states."""
-    last = _new_state(cu, k, v) if want_state else None
-    sizes = _sizes(q, k, v, cu)
+    last = _new_state(cu, plan, q) if want_state else None
+    sizes = (cu.numel() - 1, *plan.sizes)
     nws = workspace_bytes(*sizes, False)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    strides = plan.strides if planned and out.is_contiguous() else _strides((q, k, v, out))
     _ffi.launch(_ffi.lib().scree_linear_attn_fwd, q, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 log_decay.data_ptr(), out.data_ptr(), _ffi.ptr(init), _ffi.ptr(last), cu.data_ptr(),
-                *sizes, _strides((q, k, v, out)), scale, _ffi.dtype_code(q.dtype), _ffi.ptr(ws), nws)
+                *sizes, strides, scale, plan.code, _ffi.ptr(ws), nws)
     return last, ws
 
 
-# The backward runs on autograd's own thread, where Python costs several times
-# what it does here: what the forward knows of the call (sizes, the strides of
-# a contiguous gradient) is laid out by it.
-def _bwd_plan(q, k, v, cu):
-    n, h, _ = q.shape
-    dv = v.shape[2]
-    rows = [_row_head(t) for t in (q, k, v)]
-    fresh = [(t.shape[1] * t.shape[2], t.shape[2]) for t in (q, k, v)]
-    return (_sizes(q, k, v, cu),
-            _ffi.int64_array(sum([(h * dv, dv), *rows, *fresh], ())),
-            _ffi.dtype_code(q.dtype))
-
-
-def linear_bwd(do, q, k, v, log_decay, cu, scale, init, dlast, want_dinit, fwd_ws=None, plan=None):
+def linear_bwd(plan, planned, do, q, k, v, log_decay, cu, scale, init, dlast, want_dinit,
+               fwd_ws=None):
     dq, dk, dv = _like(q), _like(k), _like(v)
-    dinit = _new_state(cu, k, v) if want_dinit else None
-    sizes, strides, code = _bwd_plan(q, k, v, cu) if plan is None else plan
-    if not do.is_contiguous():
-        strides = _strides((do, q, k, v, dq, dk, dv))
+    dinit = _new_state(cu, plan, q) if want_dinit else None
+    sizes = (cu.numel() - 1, *plan.sizes)
+    strides = (plan.bwd_strides if planned and do.is_contiguous()
+               else _strides((do, q, k, v, dq, dk, dv)))
     nws = workspace_bytes(*sizes, fwd_ws is None)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
     _ffi.launch(_ffi.lib().scree_linear_attn_bwd, q, do.data_ptr(), q.data_ptr(), k.data_ptr(),
                 v.data_ptr(), log_decay.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                 _ffi.ptr(init), _ffi.ptr(dlast), _ffi.ptr(dinit), _ffi.ptr(fwd_ws), cu.data_ptr(),
-                *sizes, strides, scale, code, _ffi.ptr(ws), nws)
+                *sizes, strides, scale, plan.code, _ffi.ptr(ws), nws)
     return dq, dk, dv, dinit
 
 
 class _LinearAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, cu, scale, init, want_state):
-        qk, kk, vk, s0 = _view(q), _view(k), _view(v), _state(init)
-        out = torch.empty((*q.shape[:2], v.shape[2]), dtype=q.dtype, device=q.device)
+    def forward(ctx, q, k, v, log_decay, cu, scale, init, want_state, plan):
+        qk, kk, vk, planned = _read(plan, q, k, v)
+        s0 = _state(init)
+        out = q.new_empty(plan.out_shape)
         # the workspace's states between segments serve the backward too
-        last, ws = linear_fwd(qk, kk, vk, log_decay, cu, scale, s0, want_state, out)
+        last, ws = linear_fwd(plan, planned, qk, kk, vk, log_decay, cu, scale, s0, want_state, out)
         ctx.save_for_backward(qk, kk, vk, log_decay, cu, s0, ws)
-        ctx.scale = scale
-        ctx.plan = _bwd_plan(qk, kk, vk, cu)
+        ctx.call = plan, planned, scale
         ctx.set_materialize_grads(False)
         return (out, last) if want_state else out
 
@@ -194,22 +211,23 @@ class _LinearAttentionFn(torch.autograd.Function):
     def backward(ctx, do, dlast=None):
         q, k, v, log_decay, cu, s0, ws = ctx.saved_tensors
         if do is None and dlast is None:
-            return (None,) * 8
+            return (None,) * 9
+        plan, planned, scale = ctx.call
         if do is None:
-            do = torch.zeros((*q.shape[:2], v.shape[2]), dtype=q.dtype, device=q.device)
-        grads = linear_bwd(_view(do), q, k, v, log_decay, cu, ctx.scale, s0, _state(dlast),
-                           ctx.needs_input_grad[6], ws, ctx.plan)
+            do = q.new_zeros(plan.out_shape)
+        grads = linear_bwd(plan, planned, _view(do), q, k, v, log_decay, cu, scale, s0, _state(dlast),
+                           ctx.needs_input_grad[6], ws)
         dq, dk, dv, dinit = once("varlen linear attention", *grads)
-        return dq, dk, dv, None, None, None, dinit, None
+        return dq, dk, dv, None, None, None, dinit, None, None
 
 
 def _prepare(q, k, v, log_decay, cu_seqlens, scale, initial_state):
-    _, default_scale = _check(q, k, v, log_decay)
+    plan = _check(q, k, v, log_decay)
     cu = _cu(cu_seqlens, q.device)
     assert cu.dim() == 1 and cu.numel() >= 2, "cu_seqlens must have batch + 1 entries"
     if initial_state is not None:
         _check_state(initial_state, "initial_state", cu.numel() - 1, k, v)
-    return cu, default_scale if scale is None else float(scale)
+    return plan, cu, plan.scale if scale is None else float(scale)
 
 
 def varlen_linear_attention_hip(q, k, v, log_decay, cu_seqlens, scale=None, initial_state=None,
@@ -236,14 +254,15 @@ def varlen_linear_attention_hip(q, k, v, log_decay, cu_seqlens, scale=None, init
 
     Returns ``out`` ``(total_tokens, heads, v_dim)`` or ``(out, state)``.
     """
-    cu, scale = _prepare(q, k, v, log_decay, cu_seqlens, scale, initial_state)
-    tracked = [t for t in (q, k, v, initial_state) if t is not None and t.requires_grad]
-    if torch.is_grad_enabled() and tracked:
+    plan, cu, scale = _prepare(q, k, v, log_decay, cu_seqlens, scale, initial_state)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (
+            initial_state is not None and initial_state.requires_grad)):
         assert out is None, "out= is not supported when an input requires grad"
         return _LinearAttentionFn.apply(q, k, v, log_decay.contiguous(), cu, scale, initial_state,
-                                        bool(return_state))
-    out, ok = _out(out, (*q.shape[:2], v.shape[2]), q, "total_tokens")
-    last, _ = linear_fwd(_view(q), _view(k), _view(v), log_decay.contiguous(), cu, scale,
+                                        bool(return_state), plan)
+    out, ok = _out(out, plan.out_shape, q, "total_tokens")
+    qk, kk, vk, planned = _read(plan, q, k, v)
+    last, _ = linear_fwd(plan, planned, qk, kk, vk, log_decay.contiguous(), cu, scale,
                          _state(initial_state), return_state, ok)
     if ok is not out:
         out.copy_(ok)
@@ -258,25 +277,39 @@ def varlen_linear_attention_hip_backward(do, q, k, v, log_decay, cu_seqlens, sca
     ``dinitial_state`` is None without an ``initial_state``.  Gradient rows
     past the last sequence are zero.
     """
-    cu, scale = _prepare(q, k, v, log_decay, cu_seqlens, scale, initial_state)
-    assert do.shape == (*q.shape[:2], v.shape[2]) and do.dtype == q.dtype and do.device == q.device, (
+    plan, cu, scale = _prepare(q, k, v, log_decay, cu_seqlens, scale, initial_state)
+    assert do.shape == plan.out_shape and do.dtype == q.dtype and do.device == q.device, (
         "do must be (total_tokens, heads, v_dim) like q")
     if dstate is not None:
         _check_state(dstate, "dstate", cu.numel() - 1, k, v)
-    return linear_bwd(_view(do), _view(q), _view(k), _view(v), log_decay.contiguous(), cu, scale,
+    qk, kk, vk, planned = _read(plan, q, k, v)
+    return linear_bwd(plan, planned, _view(do), qk, kk, vk, log_decay.contiguous(), cu, scale,
                       _state(initial_state), _state(dstate), initial_state is not None)
 
 
-def _step_state(s, name, batch, k, v):
-    _check_state(s, name, batch, k, v)
-    _, hk, dk, dv = s.shape
-    s0, s1, s2, s3 = s.stride()
+@functools.lru_cache(maxsize=512)
+def _state_row(name, shape, stride, dtype, batch, hk, dk, dv):
+    """The row stride of a decoding state of this layout."""
+    assert shape == (batch, hk, dk, dv), f"{name} must be (batch, kv_heads, k_dim, v_dim)"
+    assert dtype == torch.float32, f"{name} must be float32"
+    s0, s1, s2, s3 = stride
     if batch <= 1:
         s0 = hk * dk * dv
     assert (s1 == dk * dv or hk == 1) and s2 == dv and s3 == 1 and s0 % 4 == 0 and (
-        s0 >= hk * dk * dv) and s.data_ptr() % 16 == 0, (
-        f"{name} must hold each row's state contiguously, 16-byte aligned")
+        s0 >= hk * dk * dv), f"{name} must hold each row's state contiguously"
     return s0
+
+
+def _step_state(s, name, q, sizes):
+    assert s.get_device() == q.get_device(), f"{name} must be on q's device"
+    row = _state_row(name, s.shape, s.stride(), s.dtype, sizes[0], *sizes[2:])
+    assert s.data_ptr() % 16 == 0, f"{name} must be 16-byte aligned"
+    return row
+
+
+@functools.lru_cache(maxsize=512)
+def _step_strides(rows, *state_rows):
+    return _ffi.int64_array(rows + state_rows)
 
 
 def linear_attention_step_hip(q, k, v, log_decay, state, scale=None, state_out=None, out=None):
@@ -290,26 +323,28 @@ def linear_attention_step_hip(q, k, v, log_decay, state, scale=None, state_out=N
     ``(batch, heads, v_dim)``; one step of what
     :func:`varlen_linear_attention_hip` computes.  No gradient is recorded.
     """
-    code, default_scale = _check(q, k, v, log_decay)
+    plan = _check(q, k, v, log_decay)
     assert not ((q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)
                 and torch.is_grad_enabled()), (
         "a decoding step records no gradient; use varlen_linear_attention_hip")
-    b, h, dk = q.shape
-    hk, dv = v.shape[1:]
-    rows = _step_state(state, "state", b, k, v)
+    rows = rows_out = _step_state(state, "state", q, plan.sizes)
     if state_out is None:
-        state_out, rows_out = state, rows
+        state_out = state
     else:
-        rows_out = _step_state(state_out, "state_out", b, k, v)
-    out, ok = _out(out, (b, h, dv), q, "batch")
-    if b == 0:
+        rows_out = _step_state(state_out, "state_out", q, plan.sizes)
+    out, ok = _out(out, plan.out_shape, q, "batch")
+    if plan.sizes[0] == 0:
         return out
     increment_version(state_out)
-    qk, kk, vk = _view(q), _view(k), _view(v)
+    qk, kk, vk, planned = _read(plan, q, k, v)
+    if planned and ok.is_contiguous():
+        strides = _step_strides(plan.rows, rows, rows_out)
+    else:
+        strides = _strides((qk, kk, vk, ok), (rows, rows_out))
     _ffi.launch(_ffi.lib().scree_linear_attn_step, qk, qk.data_ptr(), kk.data_ptr(), vk.data_ptr(),
                 log_decay.contiguous().data_ptr(), ok.data_ptr(), state.data_ptr(),
-                state_out.data_ptr(), b, h, hk, dk, dv, _strides((qk, kk, vk, ok), (rows, rows_out)),
-                default_scale if scale is None else float(scale), code)
+                state_out.data_ptr(), *plan.sizes, strides,
+                plan.scale if scale is None else float(scale), plan.code)
     if ok is not out:
         out.copy_(ok)
     return out
