@@ -155,6 +155,55 @@ __device__ __forceinline__ void offer(TopList& l, float v, int i, int top_k) {
   }
 }
 
+// The lanes' (v, i) for which `reach` holds, behind the `count` already there
+// (those past `room` are counted only).
+__device__ __forceinline__ void append(float2* found, int room, int& count, bool reach, float v, int i) {
+  const uint64_t mask = __ballot(reach);
+  const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+  if (reach && at < room) found[at] = make_float2(v, __builtin_bit_cast(float, i));
+  count += __popcll(mask);
+}
+// The (v, i) of N arrays, counts[n] <= 64 each, into an empty list: each counts
+// those ahead of it.  By one wave; `order` has 64 places.
+template <int N>
+__device__ __forceinline__ void rank_into(TopList& l, const float2 (*found)[64], const int (&counts)[N],
+                                          float2* order, int top_k) {
+  const int lane = threadIdx.x & 63;
+  order[lane] = make_float2(-__builtin_inff(), __builtin_bit_cast(float, 0x7fffffff));
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  int total = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n) total += counts[n];
+  for (int base = 0; base < total; base += 64) {
+    int at = base + lane, from = 0;  // this lane's place, and its array
+    const bool have = at < total;
+    if (!have) at = 0;
+#pragma unroll
+    for (int n = 0; n + 1 < N; ++n)
+      if (from == n && at >= counts[n]) at -= counts[n], ++from;
+    const float2 mine = found[from][at];
+    int rank = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      for (int j = 0; j < counts[n]; ++j) {
+        const float2 o = found[n][j];
+        rank += ahead(o.x, __builtin_bit_cast(int, o.y), mine.x, __builtin_bit_cast(int, mine.y));
+      }
+    if (have && rank < top_k) order[rank] = mine;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  l.v = order[lane].x;
+  l.i = __builtin_bit_cast(int, order[lane].y);
+  const int last_i = __builtin_amdgcn_readlane(l.i, top_k - 1);
+  if (last_i != 0x7fffffff) {
+    l.last_v = lane_f(l.v, top_k - 1);
+    l.last_i = last_i;
+  }
+}
+
 // ---------------------------------------------------------------- forward
 struct LogprobOut {
   float* logprob;
@@ -204,13 +253,23 @@ __device__ __forceinline__ void finish_row(const Stats& a, const TopList& l, con
 
 // Workspace of a split forward: per part 3 floats, then per part top_k
 // (value, index) pairs.
-template <typename T, bool TOP, bool NT>
+// TOPS: how the most likely tokens are found.  A row (or part) of one trip has no
+// list to keep up: what reaches the bound is collected and ranked once, by wave 0
+// (with the join that ranks too, 16 rows x 128,000 with 20 alternatives: 17.6 us,
+// with lists 20.2; 4,096 x 5,000 with 64: 46 against 59).  A few are in their
+// lists sooner (256 x 32,000 with 5: 15.3 us against 16.4).
+constexpr int kLpFewTops = 8;
+enum Tops { kTopNone, kTopLists, kTopRanked };
+constexpr int kLpVectors = 4;  // vectors per thread and trip, their loads issued together
+template <typename T> constexpr int trip_columns() { return kLpVectors * kLpThreads * 16 / (int)sizeof(T); }
+template <typename T, Tops TOPS, bool NT>
 __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
     const T* __restrict__ logits, int64_t stride, const void* __restrict__ targets, int target_bytes,
     int vocab, int top_k, int parts, int part_cols, float* __restrict__ part_stats,
     float2* __restrict__ part_top, LogprobOut out) {
   constexpr int VEC = 16 / sizeof(T);
-  constexpr int U = 4;  // vectors per thread and trip, their loads issued together
+  constexpr int U = kLpVectors;
+  constexpr bool TOP = TOPS != kTopNone, RANKED = TOPS == kTopRanked;
   const int part = blockIdx.x % parts;
   const int64_t row = blockIdx.x / parts;
   const T* x = logits + row * stride;
@@ -223,7 +282,10 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
   TopList l;
   if constexpr (TOP) l.init();
   const int whole = c0 + (c1 - c0) / VEC * VEC;
-  __shared__ float lane_max[TOP ? kLpThreads : 1];
+  __shared__ __align__(16) float lane_max[TOP ? kLpThreads : 1];
+  __shared__ float2 found[RANKED ? kLpWaves : 1][64];
+  __shared__ int found_n[RANKED ? kLpWaves : 1];
+  int count = 0;
   // trips are uniform over a wave (its list needs every lane), the first over
   // the workgroup (its lanes' maxima bound the lists)
   int base = c0 + wave * 64 * VEC;
@@ -255,8 +317,22 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
         for (int w = 0; w < kLpWaves; ++w) mxs[w] = lane_max[64 * w + lane];
         seed(l, mxs, top_k);
       }
+      if constexpr (RANKED) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = base + u * kLpThreads * VEC + lane * VEC;
+          if (__ballot(have[u] && mx[u] >= l.last_v)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const float f = elem<T>(v[u], e);
+              append(found[wave], 64, count, have[u] && ahead(f, c + e, l.last_v, l.last_i), f, c + e);
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        if (RANKED && count <= 64) break;
         const int c = base + u * kLpThreads * VEC + lane * VEC;
         if (__ballot(have[u] && mx[u] >= l.last_v)) {
 #pragma unroll
@@ -281,6 +357,14 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
     }
     base += U * kLpThreads * VEC;
   } while (base < whole);
+  if constexpr (RANKED) {
+    if (count > 64) {  // too many: the list's
+      found[wave][lane] = make_float2(l.v, __builtin_bit_cast(float, l.i));
+      count = min(top_k, (int)__popcll(__ballot(l.i != 0x7fffffff)));
+    }
+    if (lane == 0) found_n[wave] = count;
+    l.init();
+  }
   if (wave == 0) {  // the last columns, fewer than a vector
     const bool have = whole + lane < c1;
     const float f = have ? to_f32(x[whole + lane]) : -__builtin_inff();
@@ -291,24 +375,34 @@ __global__ __launch_bounds__(kLpThreads) void logprob_fwd_kernel(
   }
 
   __shared__ float red[kLpWaves][3];
-  __shared__ float top_v[TOP ? kLpWaves : 1][kLpMaxTop];
-  __shared__ int top_i[TOP ? kLpWaves : 1][kLpMaxTop];
+  constexpr bool LISTS = TOPS == kTopLists;
+  __shared__ float top_v[LISTS ? kLpWaves : 1][kLpMaxTop];
+  __shared__ int top_i[LISTS ? kLpWaves : 1][kLpMaxTop];
   a = wave_merge(a);
   if (lane == 0) {
     red[wave][0] = a.m;
     red[wave][1] = a.s;
     red[wave][2] = a.t;
   }
-  if constexpr (TOP) {
+  if constexpr (LISTS) {
     top_v[wave][lane] = l.v;
     top_i[wave][lane] = l.i;
   }
   __syncthreads();
   if (wave != 0) return;
 #pragma unroll
-  for (int w = 1; w < kLpWaves; ++w) {
-    a = merge(a, {red[w][0], red[w][1], red[w][2]});
-    if constexpr (TOP)
+  for (int w = 1; w < kLpWaves; ++w) a = merge(a, {red[w][0], red[w][1], red[w][2]});
+  if constexpr (RANKED) {
+    int counts[kLpWaves];
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) counts[w] = __builtin_amdgcn_readfirstlane(found_n[w]);
+    const TopList rest = l;  // of the last columns
+    l.init();
+    rank_into(l, found, counts, reinterpret_cast<float2*>(lane_max), top_k);
+    offer(l, lane < VEC && rest.i != 0x7fffffff ? rest.v : __builtin_nanf(""), rest.i, top_k);
+  } else if constexpr (LISTS) {
+#pragma unroll
+    for (int w = 1; w < kLpWaves; ++w)
       offer(l, lane < top_k ? top_v[w][lane] : __builtin_nanf(""), top_i[w][lane], top_k);
   }
   if (parts > 1) {
@@ -348,14 +442,41 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(
     constexpr int R = 12;  // a lane's candidates per turn, their loads issued together
     for (int base = 0; base < n; base += 64 * R) {
       float2 c[R];
-      float mx[1] = {-__builtin_inff()};
+      constexpr int G = 4;  // groups of a lane's candidates
+      float mx[G] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const int at = base + 64 * i + lane;
         c[i] = at < n ? pt[at] : make_float2(__builtin_nanf(""), 0.f);
-        mx[0] = fmaxf(mx[0], c[i].x);
+        mx[i % G] = fmaxf(mx[i % G], c[i].x);
       }
-      if (base == 0) seed(l, mx, top_k);
+      if (base == 0) {
+        if (top_k > 32) {  // 64 maxima bound as many little
+          seed(l, mx, top_k);
+        } else {
+          const float one[1] = {fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))};
+          seed(l, one, top_k);
+        }
+      }
+      if (top_k > kLpFewTops && n <= 64 * R) {
+        // the few that reach the bound, side by side (one after the other into
+        // the list 16 x 128,000 with 20 took 8.5 us against 6.7)
+        __shared__ float2 found[G][64], order[64];
+        int total = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const int at = __builtin_bit_cast(int, c[i].y);
+          append(found[0], 64 * G, total, ahead(c[i].x, at, l.last_v, l.last_i), c[i].x, at);
+        }
+        __syncthreads();
+        if (total <= 64 * G) {
+          int counts[G];
+#pragma unroll
+          for (int j = 0; j < G; ++j) counts[j] = min(max(total - 64 * j, 0), 64);
+          rank_into(l, found, counts, order, top_k);
+          break;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < R; ++i) offer(l, c[i].x, __builtin_bit_cast(int, c[i].y), top_k);
     }
@@ -501,8 +622,10 @@ int launch_fwd(const void* logits, int64_t stride, const void* targets, int targ
   float2* pt = parts > 1 ? reinterpret_cast<float2*>(ps + (3 * rows * parts + 3) / 4 * 4) : nullptr;
   const dim3 grid((unsigned)(rows * parts));
   const T* x = static_cast<const T*>(logits);
-  auto kernel = top_k ? (nt ? logprob_fwd_kernel<T, true, true> : logprob_fwd_kernel<T, true, false>)
-                      : (nt ? logprob_fwd_kernel<T, false, true> : logprob_fwd_kernel<T, false, false>);
+  auto kernel = top_k == 0 ? (nt ? logprob_fwd_kernel<T, kTopNone, true> : logprob_fwd_kernel<T, kTopNone, false>)
+              : top_k > kLpFewTops && cols <= trip_columns<T>()
+                  ? (nt ? logprob_fwd_kernel<T, kTopRanked, true> : logprob_fwd_kernel<T, kTopRanked, false>)
+                  : (nt ? logprob_fwd_kernel<T, kTopLists, true> : logprob_fwd_kernel<T, kTopLists, false>);
   hipLaunchKernelGGL(kernel, grid, dim3(kLpThreads), 0, stream, x, stride, targets, target_bytes, vocab,
                      top_k, parts, cols, ps, pt, out);
   if (parts > 1)

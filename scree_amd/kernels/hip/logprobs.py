@@ -32,16 +32,21 @@ class TokenLogprobs(NamedTuple):
     top_index: Optional[torch.Tensor]
 
 
-def _check(logits, targets, top_k):
-    assert logits.is_cuda, "varlen_token_logprobs on HIP requires ROCm device tensors"
-    assert logits.dim() == 2 and logits.shape[1] >= 1, "logits must be (total_tokens, vocab)"
-    assert logits.dtype in (torch.float32, torch.float16, torch.bfloat16), (
-        f"unsupported dtype {logits.dtype}")
-    assert targets.shape == logits.shape[:1], "targets must have one token per row of logits"
-    assert targets.dtype in (torch.int32, torch.int64), "targets must be int32 or int64"
-    assert targets.device == logits.device, "targets must be on the same device as logits"
-    assert 0 <= top_k <= min(MAX_TOP_K, logits.shape[1]), (
+@functools.lru_cache(maxsize=512)
+def _check_shapes(xs, dtype, ys, ydtype, top_k):
+    assert len(xs) == 2 and xs[1] >= 1, "logits must be (total_tokens, vocab)"
+    assert dtype in (torch.float32, torch.float16, torch.bfloat16), f"unsupported dtype {dtype}"
+    assert ys == xs[:1], "targets must have one token per row of logits"
+    assert ydtype in (torch.int32, torch.int64), "targets must be int32 or int64"
+    assert 0 <= top_k <= min(MAX_TOP_K, xs[1]), (
         f"top_k must be in [0, {MAX_TOP_K}] and at most the vocabulary")
+
+
+def _check(logits, targets, top_k):
+    dev = logits.get_device()
+    assert dev >= 0, "varlen_token_logprobs on HIP requires ROCm device tensors"
+    _check_shapes(logits.shape, logits.dtype, targets.shape, targets.dtype, top_k)
+    assert dev == targets.get_device(), "targets must be on the same device as logits"
 
 
 def _rows_view(x):
@@ -57,17 +62,16 @@ def _workspace_bytes(rows, vocab, top_k):
 
 def logprobs_fwd(x, targets, top_k, want_stats):
     rows, vocab = x.shape
-    dev = x.device
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    logprob = x.new_empty(rows, dtype=torch.float32)
     entropy = torch.empty_like(logprob)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     top_lp = top_i = None
     if top_k:
-        top_lp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-        top_i = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+        top_lp = x.new_empty((rows, top_k), dtype=torch.float32)
+        top_i = x.new_empty((rows, top_k), dtype=torch.int64)
     if rows:
         nbytes = _workspace_bytes(rows, vocab, top_k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _ffi.launch(_ffi.lib().scree_token_logprobs, x, x.data_ptr(), x.stride(0),
                     targets.data_ptr(), targets.element_size(), rows, vocab, top_k,
                     logprob.data_ptr(), entropy.data_ptr(), _ffi.ptr(stats), _ffi.ptr(top_lp),
@@ -87,8 +91,7 @@ def _grad_of(g, shape, x):
 
 def logprobs_bwd(x, targets, stats, entropy, top_i, dlogprob, dentropy, dtop):
     rows, vocab = x.shape
-    dx = (torch.empty_like(x) if x.is_contiguous()
-          else torch.empty((rows, vocab), dtype=x.dtype, device=x.device))
+    dx = torch.empty_like(x) if x.is_contiguous() else x.new_empty((rows, vocab))
     top_k = 0 if top_i is None else top_i.shape[1]
     grads = [_grad_of(dlogprob, (rows,), x), _grad_of(dentropy, (rows,), x),
              _grad_of(dtop, (rows, top_k), x)]

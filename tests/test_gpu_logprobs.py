@@ -302,3 +302,27 @@ def test_large_logits_take_streaming_loads():
     dw, = torch.autograd.grad(want.logprob, [part], g[rows])
     # each is one rounding of values E apart: 2 u and 2 E of themselves, and a subnormal's step
     assert ((dx[rows].float() - dw.float()).abs() <= 2 * (2.0 ** -11 + E) * dw.float().abs() + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype,trip", [(torch.bfloat16, 8192), (torch.float32, 4096)])
+@pytest.mark.parametrize("top_k", [1, 20, 64])
+def test_rows_of_one_trip_and_a_little_more(dtype, trip, top_k):
+    """Alternatives are ranked at once in rows of up to a trip of the workgroup,
+    kept in lists beyond; more than 64 candidates to a wave, and in the last columns."""
+    for vocab in (trip - 1, trip, trip + 3, trip + 200):
+        x, y = _logits(8, vocab, dtype, vocab + top_k)
+        x[1] = 2.0                                   # all equal
+        x[2] = -float("inf")
+        x[2, vocab - 3:] = torch.arange(3, dtype=dtype, device="cuda")   # the last columns alone
+        y[2] = vocab - 1
+        x[3, : vocab // 2] = 9.0                     # thousands of largest ones
+        x[4, ::64] = 9.0
+        x[5] = torch.sort(x[5].float()).values.to(dtype)
+        x[6] = torch.sort(x[6].float(), descending=True).values.to(dtype)
+        x[7, vocab - 1] = 50.0
+        _check(x, y, top_k)
+        # whole rows to a workgroup give the same
+        many = x.repeat(160, 1)
+        from scree_amd.kernels.hip import varlen_token_logprobs_hip
+        a, b = varlen_token_logprobs_hip(x, y, top_k), varlen_token_logprobs_hip(many, y.repeat(160), top_k)
+        assert torch.equal(b.top_index, a.top_index.repeat(160, 1))
